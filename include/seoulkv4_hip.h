@@ -227,6 +227,123 @@ int skv_read_dense_output(void *handle, uint16_t *host_out);
 int skv_dense_decode_static(const void *kv8, int rows, int T, const void *q_dev,
                             void *out_dev, void *stream);
 
+/* ------------------------------------------------------------------------
+ * A record cache of several sequences, held by the caller, and the operators
+ * of a decoder around it (no counterpart in the reference, whose cache is one
+ * immutable sequence with post-RoPE keys: README.md:66-69).
+ *
+ * The records are those of skv_dense_decode_static, FP8 e4m3fn [V (256 B) ||
+ * K (256 B)], in slots 0 .. capacity-1 of each sequence:
+ *   contiguous (page_tokens 0): records = [batch][4][capacity][512];
+ *   paged: records = [n_pages][4][page_tokens][512], slot t of sequence b at
+ *   slot t % page_tokens of page page_table[b][t / page_tokens]
+ *   (page_tokens a power of two in [16, 65536], capacity = table_len x
+ *   page_tokens).
+ * page_table, lengths and every other array are device memory of the current
+ * device, read when the kernels run, so a captured call follows their values.
+ * lengths[b] counts the committed slots; values outside [0, capacity] count
+ * as the nearest bound.  A page_table entry outside [0, n_pages) stands for
+ * no page: its keys are invisible and writes to it are dropped.
+ *
+ * Every call enqueues on `stream` (NULL = the default stream) without
+ * synchronising or allocating, and returns SKV_EINVAL, nothing enqueued, for
+ * sizes, alignments or memory that it cannot take (skv_last_error(NULL) has
+ * the text).  Two calls may overlap unless one of them writes what the other
+ * reads or both have one workspace. */
+typedef struct {
+  void *records;               /* 16-byte aligned */
+  int32_t batch;               /* sequences, 1 .. 1024 */
+  int32_t capacity;            /* slots per sequence, 1 .. 2^20 */
+  int64_t n_pages;             /* paged: pages in records, else 0 */
+  int32_t page_tokens;         /* paged: tokens per page, else 0 */
+  int32_t table_len;           /* paged: page_table entries per sequence, else 0 */
+  const int32_t *page_table;   /* paged: [batch][table_len], else NULL */
+  int32_t *lengths;            /* [batch] */
+  int32_t *positions;          /* [batch][4][capacity] position of each slot's token, or NULL */
+  float *weights;              /* [batch][4][capacity] accumulated attention weight, or NULL */
+  int32_t *status;             /* [1], bits set by kernels and never cleared: 1 a token
+                                  past the capacity was dropped, 2 one without a page; or NULL */
+} skv_record_cache;
+
+/* Rows [batch][n][heads][dim] of a tensor: strides in elements, the last
+ * dimension contiguous. */
+typedef struct {
+  const void *data;
+  int64_t batch_stride, token_stride, head_stride;
+} skv_rows;
+
+/* Rotary positions: pair i of a head is turned by the angle
+ * 2 pi turns[i] / 2^64 per position.  Pair i is elements (i, pairs + i), or
+ * (2i, 2i + 1) with interleaved; elements past 2 x pairs are not turned. */
+typedef struct {
+  const uint64_t *turns;       /* device [pairs] */
+  int32_t pairs;               /* 1 .. 512 */
+  int32_t interleaved;
+  float scale;                 /* factor on the turned elements */
+} skv_rotary_table;
+
+enum { SKV_BF16 = 0, SKV_FP16 = 1, SKV_FP32 = 2 };
+
+/* y = the rows x [batch][n][heads][dim] turned to their positions: for a pair
+ * (a, b) at angle t, scale x (a cos t - b sin t, b cos t + a sin t); with
+ * transpose the transposed map (the gradient with respect to x for a gradient
+ * y).  FP32 arithmetic from 64-bit angles, one rounding to dtype.  dim <=
+ * 1024; positions: device [n] (position_batch_stride 0) or [batch] rows of n
+ * at that stride, int32 or int64.  y may be x with the same strides;
+ * otherwise they must not overlap. */
+int skv_rotary(const skv_rotary_table *table, const skv_rows *x, const skv_rows *y, int dtype,
+               int batch, int n, int heads, int dim, const void *positions,
+               int64_t position_batch_stride, int positions64, int transpose, void *stream);
+
+/* Writes n new tokens of every sequence into slots lengths[b] .. +n-1: V and
+ * the turned K as FP8 records (one rounding from FP32), the position and a
+ * zero weight where the cache has those arrays.  k, v: BF16 rows [batch][n][4]
+ * [256].  table NULL: K is stored as given.  q (NULL: none): BF16 rows
+ * [batch][n][16][256], turned like K into q_out, BF16 rows that may be q.
+ * positions NULL: token i of sequence b has position lengths[b] + i; else
+ * device [batch][n], int32 or int64.  counts NULL: n tokens each; else device
+ * [batch], tokens i >= counts[b] are not written (their q_out is still
+ * defined).  lengths does not change: tokens are drafts until the caller
+ * raises it. */
+int skv_cache_write(const skv_record_cache *cache, const skv_rotary_table *table,
+                    const skv_rows *k, const skv_rows *v, const skv_rows *q, const skv_rows *q_out,
+                    int n, const void *positions, int positions64, const int32_t *counts,
+                    void *stream);
+
+/* Attention of n <= 64 drafted tokens of every sequence over its cache.  Row i
+ * sees every committed slot [0, lengths[b]) and the draft slots lengths[b] + j
+ * with j < min(n, counts[b]) and bit j of tree[b][i] set (tree NULL: j <= i, a
+ * chain); rows i >= counts[b] see nothing.  q: BF16 rows [batch][n][16][256];
+ * score s = q.k / 16, with cap > 0 cap tanh(s / cap); out: BF16
+ * [batch][n][16][256] = softmax(s) V, lse: FP32 [batch][n][16] = log sum exp
+ * s; a row that sees nothing gives 0 and -inf.  workspace: device memory,
+ * 16-byte aligned, of skv_tree_workspace(batch, n) bytes. */
+int skv_tree_decode(const skv_record_cache *cache, const skv_rows *q, int n, const int64_t *tree,
+                    const int32_t *counts, float cap, void *out, float *lse, void *workspace,
+                    int64_t workspace_bytes, void *stream);
+int64_t skv_tree_workspace(int batch, int n);
+
+/* The attention weight of the rows of skv_tree_decode (same arguments and
+ * visibility; lse: its output) on every key: weights[b][g][t], t < lengths[b]
+ * + min(n, counts[b]), becomes sum over the rows and the 4 heads of group g
+ * of exp(s - lse), added to its value with accumulate.  Rows with lse = -inf
+ * add nothing. */
+int skv_key_weights(const skv_record_cache *cache, const skv_rows *q, int n, const float *lse,
+                    const int64_t *tree, const int32_t *counts, float cap, int accumulate,
+                    void *stream);
+
+/* Copies what stays of every sequence and KV head into slots 0 .. m-1 of
+ * another cache `to` (same batch, capacity >= keep, other memory), in slot
+ * order: m = min(lengths[b], keep) slots, the first `sink` and the last
+ * `local` committed ones and of the rest those with the largest weights (ties:
+ * the lowest slot; NaN counts as the least).  Positions and weights go along
+ * (where both caches have them; the source must have weights); to->lengths[b] = m.  keep >= sink + local, keep >= 1.  The
+ * source is not changed.  workspace: device memory, 16-byte aligned, of
+ * skv_evict_workspace(batch, capacity, keep) bytes. */
+int skv_evict(const skv_record_cache *cache, const skv_record_cache *to, int keep, int sink,
+              int local, void *workspace, int64_t workspace_bytes, void *stream);
+int64_t skv_evict_workspace(int batch, int capacity, int keep);
+
 /* Mean milliseconds per launch over `reps` back-to-back launches of
  * mean_ms[0] the dense partial kernel, mean_ms[1] its merge kernel and
  * mean_ms[2] both (one dense decode).  Needs one skv_dense_decode first. */

@@ -70,6 +70,40 @@ class KVPagesDesc(ctypes.Structure):
     ]
 
 
+class RecordCacheDesc(ctypes.Structure):
+    _fields_ = [
+        ("records", ctypes.c_void_p),
+        ("batch", ctypes.c_int32),
+        ("capacity", ctypes.c_int32),
+        ("n_pages", ctypes.c_int64),
+        ("page_tokens", ctypes.c_int32),
+        ("table_len", ctypes.c_int32),
+        ("page_table", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("weights", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class RowsDesc(ctypes.Structure):
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("batch_stride", ctypes.c_int64),
+        ("token_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+    ]
+
+
+class RotaryDesc(ctypes.Structure):
+    _fields_ = [
+        ("turns", ctypes.c_void_p),
+        ("pairs", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+    ]
+
+
 TRACE_LIB_PATH = LIB_PATH.with_name("libseoulkv4_hip_trace.so")
 
 _lib = None
@@ -130,6 +164,13 @@ def _bind(lib: ctypes.CDLL) -> ctypes.CDLL:
         "skv_append_device": (i32, [vp, vp, vp, i32]),
         "skv_dense_decode": (i32, [vp]),
         "skv_dense_decode_static": (i32, [vp, i32, i32, vp, vp, vp]),
+        "skv_rotary": (i32, [vp, vp, vp, i32, i32, i32, i32, i32, vp, i64, i32, i32, vp]),
+        "skv_cache_write": (i32, [vp, vp, vp, vp, vp, vp, i32, vp, i32, vp, vp]),
+        "skv_tree_decode": (i32, [vp, vp, i32, vp, vp, ctypes.c_float, vp, vp, vp, i64, vp]),
+        "skv_tree_workspace": (i64, [i32, i32]),
+        "skv_key_weights": (i32, [vp, vp, i32, vp, vp, vp, ctypes.c_float, i32, vp]),
+        "skv_evict": (i32, [vp, vp, i32, i32, i32, vp, i64, vp]),
+        "skv_evict_workspace": (i64, [i32, i32, i32]),
         "skv_dense_output_device": (i32, [vp, ctypes.POINTER(vp)]),
         "skv_read_dense_output": (i32, [vp, vp]),
         "skv_time_dense": (i32, [vp, i32, vp]),
@@ -179,6 +220,45 @@ def dense_decode_static(kv8: torch.Tensor, context: int, q: torch.Tensor,
     if code != 0:
         msg = lib.skv_last_error(None).decode()
         raise RuntimeError(f"skv_dense_decode_static failed ({ERRORS.get(code, code)}): {msg}")
+
+
+class on_device:
+    """``with on_device(dev) as stream``: ``dev`` is the current device and
+    ``stream`` PyTorch's current stream there, for a call without a handle."""
+
+    __slots__ = ("index", "_guard")
+
+    def __init__(self, device: torch.device):
+        self.index = torch.cuda.current_device() if device.index is None else device.index
+        self._guard = None
+
+    def __enter__(self):
+        if torch.cuda.current_device() != self.index:
+            self._guard = torch.cuda.device(self.index)
+            self._guard.__enter__()
+        return torch.cuda.current_stream(self.index).cuda_stream or None
+
+    def __exit__(self, *exc):
+        if self._guard is not None:
+            self._guard.__exit__(*exc)
+
+
+def check_call(what: str, code: int) -> None:
+    """Raise for a failed call without a handle: ``ValueError`` for arguments
+    it refused, ``RuntimeError`` for anything else."""
+    if code != 0:
+        msg = load_library().skv_last_error(None).decode()
+        raise (ValueError if code == 1 else RuntimeError)(f"{what} failed ({ERRORS.get(code, code)}): {msg}")
+
+
+def pointer(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def rows_desc(t: torch.Tensor) -> RowsDesc:
+    """``skv_rows`` of [batch, n, heads, dim] or [n, heads, dim]."""
+    s = t.stride()
+    return RowsDesc(t.data_ptr(), s[0] if len(s) == 4 else 0, s[-3], s[-2])
 
 
 def _ptr(a: np.ndarray) -> int:

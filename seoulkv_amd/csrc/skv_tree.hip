@@ -1,0 +1,732 @@
+// Attention of drafted tokens over a record cache, and the attention weight
+// of its keys (interfaces in skv_cache.h).
+//
+// Rows: the 4 query heads of KV head g for each of n drafts, row 4 i + h.  A
+// wave holds 16 RT of them as matrix-core columns and walks pairs of 16-key
+// tiles.  Scores: K is widened from FP8 to BF16 (exact) and multiplied by the
+// BF16 queries as they are.  (FP8 products of 128 dims at a time would take K
+// as stored, but that instruction drops bits of small products: sums of 256
+// were off by up to 9e-6 of the sum of magnitudes, BF16 ones by none.)
+// Sums: the lane that holds a score also needs it as column operand of
+// softmax x V, so nothing moves between lanes; V is widened to FP16 (exact)
+// and a probability is rounded once to FP16 (half a step of 2^-10; the running
+// maximum sits at 2^7 .. 2^15, so terms down to 2^-31 of it count).  Sums,
+// maxima and row totals are FP32.
+//
+// The sequences' pairs lie in one row, cut into equal shares, one per block:
+// a batch of ragged sequences loads every CU alike.  A share that spans
+// sequences leaves one partial in each; k_tree_merge joins a sequence's.
+#include "skv_cache.h"
+#include "skv_device.h"
+#include "skv_tile.h"
+
+namespace skv {
+
+namespace {
+
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+
+constexpr int TR_PAIR = 32;      // keys per step of a wave
+constexpr int TR_BLOCKS = 64;    // shares per KV head: one block per CU
+constexpr float TR_LN2 = 0.6931471805599453f;
+// Scaled probabilities are 2^(z - m), z in log2 units, and m is moved to 7
+// below a row's largest score when one exceeds m by more than 15.
+constexpr float TR_BASE = 7.f, TR_MOST = 15.f;
+
+// What a sequence has: rows of drafts, slots that some row may see.
+struct Sequence {
+  int len, drafts, keys, rows;
+  __device__ Sequence(const CacheView& c, const int* counts, int n, int b) {
+    len = c.length(b);
+    const int k = counts ? min(max(counts[b], 0), n) : n;
+    rows = H * k;
+    drafts = min(k, c.capacity - len);
+    keys = len + drafts;
+  }
+  // The same in scalar registers, for a sequence that the whole wave is at.
+  __device__ Sequence uniform() const {
+    Sequence s = *this;
+    s.len = __builtin_amdgcn_readfirstlane(len);
+    s.drafts = __builtin_amdgcn_readfirstlane(drafts);
+    s.keys = __builtin_amdgcn_readfirstlane(keys);
+    s.rows = __builtin_amdgcn_readfirstlane(rows);
+    return s;
+  }
+};
+
+// s_start[b]: pairs of the sequences before b; s_start[batch]: all.  With
+// WHOLE a sequence without rows counts too.
+template <bool WHOLE>
+__device__ __forceinline__ int sequence_starts(const CacheView& c, const int* counts, int n, int* s_start) {
+  if (threadIdx.x < WAVE) {
+    int carry = 0;
+    for (int b0 = 0; b0 < c.batch; b0 += WAVE) {
+      const int b = b0 + threadIdx.x;
+      int pairs = 0;
+      if (b < c.batch) {
+        const Sequence s(c, counts, n, b);
+        if (WHOLE || s.rows) pairs = (s.keys + TR_PAIR - 1) / TR_PAIR;
+      }
+      const int inc = wave_incl_scan(pairs);
+      if (b < c.batch) s_start[b] = carry + inc - pairs;
+      carry += __builtin_amdgcn_readlane(inc, WAVE - 1);
+    }
+    if (threadIdx.x == 0) s_start[c.batch] = carry;
+  }
+  __syncthreads();
+  return __builtin_amdgcn_readfirstlane(s_start[c.batch]);
+}
+
+// Block k's share of `total` pairs begins here (k of `blocks`, blocks <= total).
+__host__ __device__ __forceinline__ int share_start(int total, int blocks, int k) {
+  return (int)((int64_t)total * k / blocks);
+}
+// The share that holds pair p.
+__device__ __forceinline__ int share_of(int total, int blocks, int p) {
+  return (int)((((int64_t)p + 1) * blocks - 1) / total);
+}
+
+// The sequence that holds pair p: the last one that starts at or before it.
+__device__ __forceinline__ int sequence_of(const int* s_start, int batch, int p) {
+  int lo = 0, hi = batch;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (s_start[mid] <= p) lo = mid;
+    else hi = mid;
+  }
+  return __builtin_amdgcn_readfirstlane(lo);
+}
+
+// The 16 keys from slot t on (t a multiple of 16): where they lie, the last of
+// them in reach, and whether their page is none: they are invisible then, the
+// pool's first 16 records are read in their place.
+struct Tile {
+  const uint8_t* at;
+  int last;
+  bool bad;
+};
+__device__ __forceinline__ Tile tile_at(const CacheView& c, int b, int g, int t, int keys) {
+  const int ta = min(t, (keys - 1) & ~15);  // a second tile past the end is the last again, masked
+  Tile x;
+  x.last = min(15, keys - 1 - ta);
+  x.bad = false;
+  if (c.table) {
+    const uint32_t page = (uint32_t)__builtin_amdgcn_readfirstlane((int)c.page(b, ta));
+    x.bad = page >= c.n_pages;
+    x.at = c.records + (x.bad ? 0 : c.row_in(page, g, ta) * 512);
+  } else {
+    x.at = c.records + c.row(b, g, ta) * 512;
+  }
+  return x;
+}
+
+__device__ __forceinline__ void load_k(uint4 (&k)[4], const Tile& x, int lane) {
+  const uint32_t at = min(lane & 15, x.last) * 512 + (lane >> 4) * 16;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) k[j] = *reinterpret_cast<const uint4*>(x.at + 256 + 64 * j + at);
+}
+__device__ __forceinline__ void load_v(uint4 (&v)[4], const Tile& x, int lane) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    v[r] = load_stream(x.at + (uint32_t)(min(4 * (lane >> 4) + r, x.last) * 512 + 16 * (lane & 15)));
+}
+
+// ---------------------------------------------------------------- queries
+// The score step's column operands of 16 rows: [step][lane] 16 bytes, the dims
+// step_dim(step, kb) .. +7 of row col for lane 16 kb + col.
+constexpr int STEPS = D / 32;
+constexpr int IMG_TILE = STEPS * WAVE;  // uint4 per 16 rows
+
+// Step 2 j + half takes the dims that half `half` of a lane's K word j holds.
+__device__ __forceinline__ int step_dim(int step, int kb) {
+  return 64 * (step >> 1) + 16 * kb + 8 * (step & 1);
+}
+
+// Copies the rows of a sequence into the image of `tiles` tiles; rows past
+// `rows` are 0.
+template <int THREADS>
+__device__ __forceinline__ void stage_queries(const Rows& q, int b, int g, int tiles, int rows, uint4* img) {
+  for (int at = threadIdx.x; at < tiles * IMG_TILE; at += THREADS) {
+    const int lane = at & 63, step = (at >> 6) & (STEPS - 1), row = (at / IMG_TILE) * 16 + (lane & 15);
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (row < rows)
+      w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(q.data) + b * q.sb +
+                                          (row / H) * q.st + (g * H + row % H) * q.sh +
+                                          step_dim(step, lane >> 4));
+    img[at] = w;
+  }
+}
+
+template <bool HI>
+__device__ __forceinline__ v2bf fp8_bf16x2(uint32_t w) {
+  return __builtin_bit_cast(v2bf, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 1.f, HI));
+}
+
+// The row operand of a step from its 8 FP8 bytes.
+__device__ __forceinline__ v8bf k_operand(uint32_t lo, uint32_t hi) {
+  const v2bf p[4] = {fp8_bf16x2<false>(lo), fp8_bf16x2<true>(lo), fp8_bf16x2<false>(hi), fp8_bf16x2<true>(hi)};
+  return v8bf{p[0][0], p[0][1], p[1][0], p[1][1], p[2][0], p[2][1], p[3][0], p[3][1]};
+}
+
+// q . k of two tiles of 16 keys (lane: keys 4 kb + r) for RT tiles of 16 rows
+// (lane: row col).
+template <int RT>
+__device__ __forceinline__ void scores(const uint4 (&k)[2][4], const uint4* img, int lane, v4f (&acc)[RT][2]) {
+  // the image is read from LDS for every pair: held in registers it would
+  // leave too few for the records in flight
+  asm volatile("" : "+v"(lane));
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) acc[rt][0] = acc[rt][1] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int step = 0; step < STEPS; ++step) {
+    v8bf a[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const uint4 w = k[x][step >> 1];
+      a[x] = (step & 1) ? k_operand(w.z, w.w) : k_operand(w.x, w.y);
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const v8bf q = __builtin_bit_cast(v8bf, img[rt * IMG_TILE + step * WAVE + lane]);
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        acc[rt][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[x], q, acc[rt][x], 0, 0, 0);
+    }
+    if (step & 1) __builtin_amdgcn_sched_barrier(0);  // two steps' operands live at a time
+  }
+}
+
+// tanh to about an ulp: a polynomial near 0, where 1 - 2 / (e^2x + 1) cancels.
+__device__ __forceinline__ float tanh_near(float x) {
+  const float ax = fabsf(x), x2 = x * x;
+  const float e = __builtin_amdgcn_exp2f(ax * (2.f * DN_LOG2E));
+  const float t = copysignf(fmaf(-2.f, __builtin_amdgcn_rcpf(e + 1.f), 1.f), x);
+  const float p = fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
+  return ax < 0.3f ? x * p : t;
+}
+
+// A score in log2 units from q . k: x in, with a cap x out tanh of that.
+struct ScoreScale {
+  float in, out;
+  __device__ ScoreScale(float cap) {
+    in = cap > 0.f ? 0.0625f / cap : 0.0625f * DN_LOG2E;
+    out = cap * DN_LOG2E;
+  }
+  template <bool CAP>
+  __device__ __forceinline__ float apply(float s) const {
+    if constexpr (CAP) return out * tanh_near(s * in);
+    return s * in;
+  }
+};
+
+// Drafts that row 4 i + h of a sequence sees, one bit each.
+__device__ __forceinline__ uint64_t row_mask(const int64_t* tree, int n, int b, int i) {
+  if (tree) return (uint64_t)tree[(size_t)b * n + i];
+  return ((2ull << i) - 1ull);
+}
+
+// Whether the key in slot t is visible to a row with mask `bits`.
+__device__ __forceinline__ bool sees(const Sequence& s, uint64_t bits, int t) {
+  const int j = t - s.len;
+  return j < 0 || (j < s.drafts && ((bits >> j) & 1ull));
+}
+
+// 0x80 in every byte of w that is an FP8 NaN.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
+  return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+}
+
+template <bool HI>
+__device__ __forceinline__ v2h fp8_f16x2(uint32_t w) {
+  return __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.f, HI));
+}
+
+// Row operands of softmax x V for dims 16 c + 4 w + i of lane 16 kb + c: its 8
+// keys (4 kb + r of both tiles), transposed and widened.
+__device__ __forceinline__ void v_operands(const uint4 (&v)[2][4], int w, v8h (&va)[4]) {
+  uint32_t d[2][4];  // d[a][i]: the 4 keys' bytes of dim 4 w + i
+#pragma unroll
+  for (int a = 0; a < 2; ++a) {
+    const uint32_t y[4] = {(&v[a][0].x)[w], (&v[a][1].x)[w], (&v[a][2].x)[w], (&v[a][3].x)[w]};
+    const uint32_t lo01 = __builtin_amdgcn_perm(y[1], y[0], 0x05010400u);
+    const uint32_t hi01 = __builtin_amdgcn_perm(y[1], y[0], 0x07030602u);
+    const uint32_t lo23 = __builtin_amdgcn_perm(y[3], y[2], 0x05010400u);
+    const uint32_t hi23 = __builtin_amdgcn_perm(y[3], y[2], 0x07030602u);
+    d[a][0] = __builtin_amdgcn_perm(lo23, lo01, 0x05040100u);
+    d[a][1] = __builtin_amdgcn_perm(lo23, lo01, 0x07060302u);
+    d[a][2] = __builtin_amdgcn_perm(hi23, hi01, 0x05040100u);
+    d[a][3] = __builtin_amdgcn_perm(hi23, hi01, 0x07060302u);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const v2h p[4] = {fp8_f16x2<false>(d[0][i]), fp8_f16x2<true>(d[0][i]),
+                      fp8_f16x2<false>(d[1][i]), fp8_f16x2<true>(d[1][i])};
+    va[i] = v8h{p[0][0], p[0][1], p[1][0], p[1][1], p[2][0], p[2][1], p[3][0], p[3][1]};
+  }
+}
+
+// The partials: share k of sequence b has index k + b (each next one moves
+// either k or b on by one).  [G][blocks + batch][rows][256] sums, then as many
+// (m, total) pairs, then [G][blocks + batch] flags (see k_tree_merge), then
+// the sequences' starts.
+struct Partials {
+  float* o;
+  float2* stats;
+  int* nan;
+  int* starts;
+  size_t rows, shares;  // per group
+  __host__ __device__ Partials(float* part, int batch, int n) {
+    shares = TR_BLOCKS + batch;
+    rows = shares * n * H;
+    o = part;
+    stats = reinterpret_cast<float2*>(o + rows * G * D);
+    nan = reinterpret_cast<int*>(stats + rows * G);
+    starts = nan + shares * G;
+  }
+};
+
+// ------------------------------------------------------------- attention
+// A block: KW waves along the keys x RW along the rows, RT tiles of 16 rows a
+// wave.  Registers: 64 RT sums, 32 of K, 32 of V a lane.
+template <int RT, int RW, int KW, bool CAP>
+__global__ __launch_bounds__(RW * KW * 64) void k_tree(TreeArgs a) {
+  constexpr int WAVES = RW * KW, TILES = RT * RW;
+  constexpr int JOIN = (KW / 2) * RW * RT * 16 * WAVE;  // float4: waves that hand over their sums
+  constexpr int IMG = TILES * IMG_TILE;
+  __shared__ uint4 s_buf[IMG > JOIN ? IMG : JOIN];  // the queries' image, then the sums in transit
+  __shared__ float2 s_ml[(KW / 2 + 1) * RW * RT * WAVE];
+  __shared__ uint64_t s_bits[TILES * 16];
+  __shared__ int s_start[CACHE_MAX_BATCH + 1];
+  __shared__ int s_nan;
+  const int g = blockIdx.y, k = blockIdx.x;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rw = wave % RW, kw = wave / RW, col = lane & 15, kb = lane >> 4;
+  const Partials part(a.part, a.c.batch, a.n);
+  const int total = sequence_starts<false>(a.c, a.counts, a.n, s_start);
+  if (k == 0 && g == 0)
+    for (int b = threadIdx.x; b <= a.c.batch; b += WAVES * 64) part.starts[b] = s_start[b];
+  const int blocks = min((int)gridDim.x, total);
+  if (k >= blocks) return;
+  const int end = share_start(total, blocks, k + 1);
+
+  for (int p0 = share_start(total, blocks, k); p0 < end;) {
+    const int b = sequence_of(s_start, a.c.batch, p0);
+    const int first = __builtin_amdgcn_readfirstlane(s_start[b]);
+    const int p1 = min(end, __builtin_amdgcn_readfirstlane(s_start[b + 1]));
+    const Sequence seq = Sequence(a.c, a.counts, a.n, b).uniform();
+    stage_queries<WAVES * 64>(a.q, b, g, TILES, seq.rows, s_buf);
+    for (int r = threadIdx.x; r < TILES * 16; r += WAVES * 64)
+      s_bits[r] = r < seq.rows ? row_mask(a.tree, a.n, b, r / H) : 0;
+    if (threadIdx.x == 0) s_nan = 0;
+    auto tiles = [&](int pair, Tile& x, Tile& y) {
+      const int t = (pair - first) * TR_PAIR;
+      x = tile_at(a.c, b, g, t, seq.keys);
+      y = tile_at(a.c, b, g, t + 16, seq.keys);
+    };
+    int j = p0 + kw;
+    uint4 kx[2][4], vx[2][4];
+    Tile t0, t1;
+    if (j < p1) {
+      tiles(j, t0, t1);
+      load_k(kx[0], t0, lane);
+      load_k(kx[1], t1, lane);
+      load_v(vx[0], t0, lane);
+      load_v(vx[1], t1, lane);
+    }
+    __syncthreads();
+
+    v4f o[RT][16];
+    float m[RT], l[RT];
+    const ScoreScale zs(a.cap);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[rt][i] = v4f{0.f, 0.f, 0.f, 0.f};
+      m[rt] = -INFINITY;
+      l[rt] = 0.f;
+    }
+#pragma nounroll
+    for (; j < p1; j += KW) {
+      const int at = (j - first) * TR_PAIR;
+      const bool more = j + KW < p1;
+      const bool bad0 = t0.bad, bad1 = t1.bad;
+      // some of the keys are drafts, past the end or in no page
+      const bool edge = at + TR_PAIR > seq.len || bad0 || bad1;
+      if (more) tiles(j + KW, t0, t1);
+      float z[RT][8];
+      {
+        v4f acc[RT][2];
+        scores<RT>(kx, s_buf + rw * RT * IMG_TILE, lane, acc);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) z[rt][e] = zs.template apply<CAP>(acc[rt][e >> 2][e & 3]);
+      }
+      // the scores are done before their records' registers are loaded anew
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) asm volatile("" : "+v"(z[rt][e]));
+      if (more) {
+        load_k(kx[0], t0, lane);
+        load_k(kx[1], t1, lane);
+      }
+      if (edge) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          const uint64_t bits = s_bits[(rw * RT + rt) * 16 + col];
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if ((e < 4 ? bad0 : bad1) || !sees(seq, bits, at + 16 * (e >> 2) + 4 * kb + (e & 3)))
+              z[rt][e] = -INFINITY;
+        }
+      }
+      v8h pb[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        float tm = z[rt][0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) tm = fmaxf(tm, z[rt][e]);
+        if (__ballot(tm > m[rt] + TR_MOST)) {
+          tm = fmaxf(tm, __shfl_xor(tm, 16));
+          tm = fmaxf(tm, __shfl_xor(tm, 32));
+          const bool grow = tm > m[rt] + TR_MOST;
+          const float mn = grow ? tm - TR_BASE : m[rt];
+          const float al = grow ? __builtin_amdgcn_exp2f(m[rt] - mn) : 1.f;
+          l[rt] *= al;
+          m[rt] = mn;
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[rt][i][r] *= al;
+        }
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {  // (a masked key: 0, also while m = -inf)
+          const float x = __builtin_amdgcn_exp2f(z[rt][e] - m[rt]);
+          p[e] = z[rt][e] == -INFINITY ? 0.f : x;
+          pb[rt][e] = (_Float16)p[e];
+        }
+        l[rt] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+      }
+      if (edge) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (bad0) vx[0][r] = make_uint4(0, 0, 0, 0);
+          if (bad1) vx[1][r] = make_uint4(0, 0, 0, 0);
+        }
+      }
+      if (at + TR_PAIR > seq.len) {
+        // 0 x NaN would reach the rows that do not see a draft with NaN in V:
+        // such a byte counts as 0 here, and the merge puts NaN where a row
+        // sees it
+        uint32_t any = 0;
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              uint32_t& v = (&vx[x][r].x)[w];
+              const uint32_t flag = nan_bytes(v) >> 7;
+              v &= ~(flag * 0xffu);
+              any |= flag;
+            }
+        if (__ballot(any != 0) && lane == 0) s_nan = 1;
+      }
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        v8h va[4];
+        v_operands(vx, w, va);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+            o[rt][4 * w + i] =
+                __builtin_amdgcn_mfma_f32_16x16x32_f16(va[i], pb[rt], o[rt][4 * w + i], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);  // one word's operands live at a time
+      }
+      if (more) {
+        load_v(vx[0], t0, lane);
+        load_v(vx[1], t1, lane);
+      }
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      l[rt] += __shfl_xor(l[rt], 16);
+      l[rt] += __shfl_xor(l[rt], 32);
+    }
+    // the key waves' sums, halved in number by every step
+#pragma nounroll
+    for (int live = KW; live > 1; live = (live + 1) / 2) {
+      const int half = (live + 1) / 2;
+      __syncthreads();
+      if (kw >= half && kw < live) {
+        const int slot = (kw - half) * RW + rw;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            s_buf[((slot * RT + rt) * 16 + i) * WAVE + lane] = __builtin_bit_cast(uint4, o[rt][i]);
+          s_ml[(slot * RT + rt) * WAVE + lane] = make_float2(m[rt], l[rt]);
+        }
+      }
+      __syncthreads();
+      if (kw < live - half) {
+        const int slot = kw * RW + rw;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          const float2 ml = s_ml[(slot * RT + rt) * WAVE + lane];
+          const float mn = fmaxf(m[rt], ml.x);
+          // (an empty side counts 0: its m is -inf; a NaN total stays NaN)
+          const float f0 = l[rt] == 0.f ? 0.f : __builtin_amdgcn_exp2f(m[rt] - mn);
+          const float f1 = ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - mn);
+          m[rt] = mn;
+          l[rt] = fmaf(l[rt], f0, ml.y * f1);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const v4f other = __builtin_bit_cast(v4f, s_buf[((slot * RT + rt) * 16 + i) * WAVE + lane]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[rt][i][r] = fmaf(o[rt][i][r], f0, other[r] * f1);
+            if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // 4 loads in flight, not 16
+          }
+        }
+      }
+    }
+    if (kw == 0) {
+      // o[i][r] of lane (kb, col) is dim 16 (4 kb + r) + i of row col
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const int row = (rw * RT + rt) * 16 + col;
+        if (row >= seq.rows) continue;
+        const size_t at = g * part.rows + (size_t)(k + b) * a.n * H + row;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int i = 0; i < 16; i += 4)
+            *reinterpret_cast<float4*>(part.o + at * D + 16 * (4 * kb + r) + i) =
+                make_float4(o[rt][i][r], o[rt][i + 1][r], o[rt][i + 2][r], o[rt][i + 3][r]);
+        if (kb == 0) part.stats[at] = make_float2(m[rt], l[rt]);
+      }
+    }
+    p0 = p1;
+    __syncthreads();  // the buffer is formed anew
+    if (threadIdx.x == 0) part.nan[g * part.shares + k + b] = s_nan;
+  }
+}
+
+// Row (b, g, row) = blockIdx.x, dims 64 blockIdx.y + [0, 64): thread (slice,
+// 4 dims) adds partials slice, slice + 16, ...; the slices are added in order.
+// Where a share met NaN in V among the last keys (it took them as 0), those
+// keys are gone through once more and the dims in which the row sees one
+// become NaN.
+__global__ __launch_bounds__(256) void k_tree_merge(TreeArgs a, int shares) {
+  const int R = a.n * H;
+  const int row = blockIdx.x % R, g = (blockIdx.x / R) % G, b = blockIdx.x / (R * G);
+  const int dl = threadIdx.x & 15, sl = threadIdx.x >> 4, d = blockIdx.y * 64 + 4 * dl;
+  __shared__ float4 s_o[16][16];
+  __shared__ float s_m[16], s_l[16];
+  const Partials part(a.part, a.c.batch, a.n);
+  const int i = row / H, head = g * H + row % H;
+  const size_t at = ((size_t)b * a.n + i) * G * H + head;
+  const int total = part.starts[a.c.batch], start = part.starts[b], stop = part.starts[b + 1];
+  const Sequence seq(a.c, a.counts, a.n, b);
+  float m = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  int nan = 0;
+  if (row < seq.rows && start < stop) {
+    const int blocks = min(shares, total);
+    const int k1 = share_of(total, blocks, stop - 1);
+    for (int k = share_of(total, blocks, start) + sl; k <= k1; k += 16) {
+      const size_t from = g * part.rows + (size_t)(k + b) * R + row;
+      nan |= part.nan[g * part.shares + k + b];
+      const float2 ml = part.stats[from];
+      const float4 x = *reinterpret_cast<const float4*>(part.o + from * D + d);
+      const float mn = fmaxf(m, ml.x);
+      const float f0 = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+      const float f1 = ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - mn);
+      m = mn;
+      l = fmaf(l, f0, ml.y * f1);
+      o.x = fmaf(o.x, f0, x.x * f1);
+      o.y = fmaf(o.y, f0, x.y * f1);
+      o.z = fmaf(o.z, f0, x.z * f1);
+      o.w = fmaf(o.w, f0, x.w * f1);
+    }
+  }
+  s_o[sl][dl] = o;
+  if (dl == 0) {
+    s_m[sl] = m;
+    s_l[sl] = l;
+  }
+  nan = __syncthreads_or(nan);
+  if (threadIdx.x < 64) {
+    float M = -INFINITY, L = 0.f, O = 0.f;
+#pragma unroll
+    for (int s = 0; s < 16; ++s) M = fmaxf(M, s_m[s]);
+#pragma unroll
+    for (int s = 0; s < 16; ++s) {
+      const float f = s_l[s] == 0.f ? 0.f : __builtin_amdgcn_exp2f(s_m[s] - M);
+      L = fmaf(s_l[s], f, L);
+      O = fmaf((&s_o[s][threadIdx.x >> 2].x)[threadIdx.x & 3], f, O);
+    }
+    const int dim = blockIdx.y * 64 + threadIdx.x;
+    float y = L == 0.f ? 0.f : O / L;
+    if (nan) {
+      const uint64_t bits = row_mask(a.tree, a.n, b, i);
+      for (int t = seq.len & ~(TR_PAIR - 1); t < seq.keys; ++t) {
+        const uint32_t page = a.c.table ? a.c.page(b, t) : 0;
+        if (!sees(seq, bits, t) || (a.c.table && page >= a.c.n_pages)) continue;
+        const size_t record = a.c.table ? a.c.row_in(page, g, t) : a.c.row(b, g, t);
+        if ((a.c.records[record * 512 + dim] & 0x7f) == 0x7f) y = __builtin_nanf("");
+      }
+    }
+    a.out[at * D + dim] = (uint16_t)bf16_rne(y);
+    if (blockIdx.y == 0 && threadIdx.x == 0)
+      a.lse[at] = L == 0.f ? -INFINITY : (M + __log2f(L)) * TR_LN2;
+  }
+}
+
+// ------------------------------------------------------------ key weights
+// A block takes a share of the pairs of KV head g like k_tree's; its waves
+// stride the share, each with all rows of its 32 keys: the queries' image is
+// in LDS, the K halves in registers, and a key's weight is summed over the
+// rows in registers and then over the 16 lanes of a row group.
+constexpr int KWT_WAVES = 8;
+
+template <int TILES, bool CAP>
+__global__ __launch_bounds__(KWT_WAVES * 64) void k_key_weights(WeightArgs a) {
+  __shared__ uint4 s_img[TILES * IMG_TILE];
+  __shared__ float s_lse[TILES * 16];
+  __shared__ uint64_t s_bits[TILES * 16];
+  __shared__ int s_start[CACHE_MAX_BATCH + 1];
+  const int g = blockIdx.y, k = blockIdx.x;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, kb = lane >> 4;
+  const int total = sequence_starts<true>(a.c, a.counts, a.n, s_start);
+  const int blocks = min((int)gridDim.x, total);
+  if (k >= blocks) return;
+  const int end = share_start(total, blocks, k + 1);
+  for (int p0 = share_start(total, blocks, k); p0 < end;) {
+    const int b = sequence_of(s_start, a.c.batch, p0);
+    const int first = __builtin_amdgcn_readfirstlane(s_start[b]);
+    const int p1 = min(end, __builtin_amdgcn_readfirstlane(s_start[b + 1]));
+    const Sequence seq = Sequence(a.c, a.counts, a.n, b).uniform();
+    uint4 kx[2][4];
+    Tile t0, t1;
+    int j = p0 + wave;
+    auto tiles = [&](int pair, Tile& x, Tile& y) {
+      const int t = (pair - first) * TR_PAIR;
+      x = tile_at(a.c, b, g, t, seq.keys);
+      y = tile_at(a.c, b, g, t + 16, seq.keys);
+    };
+    if (j < p1) {
+      tiles(j, t0, t1);
+      load_k(kx[0], t0, lane);
+      load_k(kx[1], t1, lane);
+    }
+    stage_queries<KWT_WAVES * 64>(a.q, b, g, TILES, seq.rows, s_img);
+    for (int r = threadIdx.x; r < TILES * 16; r += KWT_WAVES * 64) {
+      const int i = r / H;
+      const bool row = r < seq.rows;
+      s_bits[r] = row ? row_mask(a.tree, a.n, b, i) : 0;
+      const float lse = row ? a.lse[((size_t)b * a.n + i) * G * H + g * H + r % H] : -INFINITY;
+      s_lse[r] = lse == -INFINITY ? INFINITY : lse * DN_LOG2E;  // (such a row adds nothing)
+    }
+    __syncthreads();
+    const int used = (seq.rows + 15) / 16;
+    const ScoreScale zs(a.cap);
+#pragma nounroll
+    for (; j < p1; j += KWT_WAVES) {
+      const int at = (j - first) * TR_PAIR;
+      const bool bad0 = t0.bad, bad1 = t1.bad;
+      const bool edge = at + TR_PAIR > seq.len || bad0 || bad1;
+      float sum[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[e] = 0.f;
+      for (int tile = 0; tile < used; ++tile) {
+        const int row = tile * 16 + col;
+        const float lse = s_lse[row];
+        v4f acc[1][2];
+        scores<1>(kx, s_img + tile * IMG_TILE, lane, acc);
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float p = __builtin_amdgcn_exp2f(zs.template apply<CAP>(acc[0][x][r]) - lse);
+            if (edge) {
+              const bool seen = !(x ? bad1 : bad0) && sees(seq, s_bits[row], at + 16 * x + 4 * kb + r);
+              p = seen ? p : 0.f;
+            }
+            sum[4 * x + r] += lse == INFINITY ? 0.f : p;
+          }
+      }
+      if (j + KWT_WAVES < p1) {
+        tiles(j + KWT_WAVES, t0, t1);
+        load_k(kx[0], t0, lane);
+        load_k(kx[1], t1, lane);
+      }
+      float mine = 0.f;  // lane col = 4 x + r of a row group keeps key 16 x + 4 kb + r
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float v = sum[e];
+        v += dpp_f<0xB1>(v);   // quad_perm [1,0,3,2]
+        v += dpp_f<0x4E>(v);   // quad_perm [2,3,0,1]
+        v += dpp_f<0x141>(v);  // row_half_mirror
+        v += dpp_f<0x140>(v);  // row_mirror
+        mine = col == e ? v : mine;
+      }
+      const int t = at + 16 * (col >> 2) + 4 * kb + (col & 3);
+      if (col < 8 && t < seq.keys) {
+        float* w = a.weights + a.c.row(b, g, t);
+        *w = a.accumulate ? *w + mine : mine;
+      }
+    }
+    p0 = p1;
+    __syncthreads();
+  }
+}
+
+template <bool CAP>
+void tree_rows(const TreeArgs& a, hipStream_t st) {
+  const dim3 grid(TR_BLOCKS, G);
+  const int tiles = (a.n * H + 15) / 16;
+  if (tiles <= 1) hipLaunchKernelGGL((k_tree<1, 1, 12, CAP>), grid, dim3(768), 0, st, a);
+  else if (tiles <= 2) hipLaunchKernelGGL((k_tree<2, 1, 8, CAP>), grid, dim3(512), 0, st, a);
+  else if (tiles <= 4) hipLaunchKernelGGL((k_tree<2, 2, 4, CAP>), grid, dim3(512), 0, st, a);
+  else if (tiles <= 8) hipLaunchKernelGGL((k_tree<2, 4, 2, CAP>), grid, dim3(512), 0, st, a);
+  else hipLaunchKernelGGL((k_tree<2, 8, 1, CAP>), grid, dim3(512), 0, st, a);
+}
+
+template <bool CAP>
+void weight_rows(const WeightArgs& a, hipStream_t st) {
+  const int tiles = (a.n * H + 15) / 16;
+  const dim3 block(KWT_WAVES * 64);
+  const dim3 grid(tiles <= 8 ? 2 * TR_BLOCKS : TR_BLOCKS, G);
+  if (tiles <= 1) hipLaunchKernelGGL((k_key_weights<1, CAP>), grid, block, 0, st, a);
+  else if (tiles <= 2) hipLaunchKernelGGL((k_key_weights<2, CAP>), grid, block, 0, st, a);
+  else if (tiles <= 4) hipLaunchKernelGGL((k_key_weights<4, CAP>), grid, block, 0, st, a);
+  else if (tiles <= 8) hipLaunchKernelGGL((k_key_weights<8, CAP>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((k_key_weights<16, CAP>), grid, block, 0, st, a);
+}
+
+}  // namespace
+
+size_t tree_workspace(int batch, int n) {
+  const Partials p(nullptr, batch, n);
+  return reinterpret_cast<size_t>(p.starts + batch + 1);
+}
+
+void launch_tree(const TreeArgs& a, hipStream_t st) {
+  (a.cap > 0.f ? tree_rows<true> : tree_rows<false>)(a, st);
+  hipLaunchKernelGGL(k_tree_merge, dim3((unsigned)(a.c.batch * G * a.n * H), D / 64), dim3(256), 0, st,
+                     a, TR_BLOCKS);
+}
+
+void launch_key_weights(const WeightArgs& a, hipStream_t st) {
+  (a.cap > 0.f ? weight_rows<true> : weight_rows<false>)(a, st);
+}
+
+}  // namespace skv
