@@ -220,6 +220,11 @@ struct ScoreScale {
     if constexpr (CAP) return out * tanh_near(s * in);
     return s * in;
   }
+  // the same less a row's log total
+  template <bool CAP>
+  __device__ __forceinline__ float less(float s, float total) const {
+    return fmaf(CAP ? tanh_near(s * in) : s, CAP ? out : in, -total);
+  }
 };
 
 // Drafts that row 4 i + h of a sequence sees, one bit each.
@@ -605,6 +610,7 @@ __global__ __launch_bounds__(KWT_WAVES * 64) void k_key_weights(WeightArgs a) {
   const int g = blockIdx.y, k = blockIdx.x;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, kb = lane >> 4;
+  const ScoreScale zs(a.cap);
   const int total = sequence_starts<true>(a.c, a.counts, a.n, s_start);
   const int blocks = min((int)gridDim.x, total);
   if (k >= blocks) return;
@@ -633,40 +639,54 @@ __global__ __launch_bounds__(KWT_WAVES * 64) void k_key_weights(WeightArgs a) {
       const bool row = r < seq.rows;
       s_bits[r] = row ? row_mask(a.tree, a.n, b, i) : 0;
       const float lse = row ? a.lse[((size_t)b * a.n + i) * G * H + g * H + r % H] : -INFINITY;
-      s_lse[r] = lse == -INFINITY ? INFINITY : lse * DN_LOG2E;  // (such a row adds nothing)
+      s_lse[r] = lse == -INFINITY ? INFINITY : lse * DN_LOG2E;  // such a row adds 2^-inf
     }
     __syncthreads();
     const int used = (seq.rows + 15) / 16;
-    const ScoreScale zs(a.cap);
 #pragma nounroll
     for (; j < p1; j += KWT_WAVES) {
       const int at = (j - first) * TR_PAIR;
       const bool bad0 = t0.bad, bad1 = t1.bad;
       const bool edge = at + TR_PAIR > seq.len || bad0 || bad1;
-      float sum[8];
+      // widened once for all rows; the records' registers are loaded anew
+      v8bf ka[2][STEPS];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum[e] = 0.f;
-      for (int tile = 0; tile < used; ++tile) {
-        const int row = tile * 16 + col;
-        const float lse = s_lse[row];
-        v4f acc[1][2];
-        scores<1>(kx, s_img + tile * IMG_TILE, lane, acc);
+      for (int x = 0; x < 2; ++x)
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            float p = __builtin_amdgcn_exp2f(zs.template apply<CAP>(acc[0][x][r]) - lse);
-            if (edge) {
-              const bool seen = !(x ? bad1 : bad0) && sees(seq, s_bits[row], at + 16 * x + 4 * kb + r);
-              p = seen ? p : 0.f;
-            }
-            sum[4 * x + r] += lse == INFINITY ? 0.f : p;
-          }
-      }
+        for (int step = 0; step < STEPS; ++step) {
+          const uint4 w = kx[x][step >> 1];
+          ka[x][step] = (step & 1) ? k_operand(w.z, w.w) : k_operand(w.x, w.y);
+        }
       if (j + KWT_WAVES < p1) {
         tiles(j + KWT_WAVES, t0, t1);
         load_k(kx[0], t0, lane);
         load_k(kx[1], t1, lane);
+      }
+      float sum[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[e] = 0.f;
+#pragma nounroll
+      for (int tile = 0; tile < used; ++tile) {
+        const int row = tile * 16 + col;
+        const float lse = s_lse[row];
+        v4f acc[2] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int step = 0; step < STEPS; ++step) {
+          const v8bf q = __builtin_bit_cast(v8bf, s_img[tile * IMG_TILE + step * WAVE + lane]);
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            acc[x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka[x][step], q, acc[x], 0, 0, 0);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float p = __builtin_amdgcn_exp2f(zs.template less<CAP>(acc[e >> 2][e & 3], lse));
+          if (edge) {
+            const bool seen = !(e < 4 ? bad0 : bad1) &&
+                              sees(seq, s_bits[row], at + 16 * (e >> 2) + 4 * kb + (e & 3));
+            p = seen ? p : 0.f;
+          }
+          sum[e] += p;
+        }
       }
       float mine = 0.f;  // lane col = 4 x + r of a row group keeps key 16 x + 4 kb + r
 #pragma unroll

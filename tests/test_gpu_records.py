@@ -378,7 +378,7 @@ def test_eviction_of_ties_and_odd_weights():
         evict_and_check(cache, keep, sink, local)
 
 
-@pytest.mark.parametrize("length", [9000, 70000, 131072])
+@pytest.mark.parametrize("length", [5000, 9000, 25000, 70000, 131072])
 def test_long_evictions(length):
     cache = make([length, 0], length + 16)
     cache.weights.copy_(torch.exp(3 * torch.randn(cache.weights.shape, generator=gen(2))).to(DEV))
