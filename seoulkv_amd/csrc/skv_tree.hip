@@ -16,6 +16,8 @@
 // The sequences' pairs lie in one row, cut into equal shares, one per block:
 // a batch of ragged sequences loads every CU alike.  A share that spans
 // sequences leaves one partial in each; k_tree_merge joins a sequence's.
+#include <type_traits>
+
 #include "skv_cache.h"
 #include "skv_device.h"
 #include "skv_tile.h"
@@ -108,13 +110,18 @@ struct Tile {
   int last;
   bool bad;
 };
+template <bool PAGED>
 __device__ __forceinline__ Tile tile_at(const CacheView& c, int b, int g, int t, int keys) {
   const int ta = min(t, (keys - 1) & ~15);  // a second tile past the end is the last again, masked
   Tile x;
   x.last = min(15, keys - 1 - ta);
   x.bad = false;
-  if (c.table) {
-    const uint32_t page = (uint32_t)__builtin_amdgcn_readfirstlane((int)c.page(b, ta));
+  if constexpr (PAGED) {
+    // a scalar load: a vector load's wait would be one for the records in
+    // flight too
+    typedef const __attribute__((address_space(4))) uint32_t* scalar;
+    const uint32_t page = reinterpret_cast<scalar>(reinterpret_cast<uintptr_t>(
+        c.table + (size_t)b * c.table_len))[ta >> c.shift];
     x.bad = page >= c.n_pages;
     x.at = c.records + (x.bad ? 0 : c.row_in(page, g, ta) * 512);
   } else {
@@ -123,15 +130,20 @@ __device__ __forceinline__ Tile tile_at(const CacheView& c, int b, int g, int t,
   return x;
 }
 
+// WHOLE: all 16 keys are in reach.
+template <bool WHOLE>
 __device__ __forceinline__ void load_k(uint4 (&k)[4], const Tile& x, int lane) {
-  const uint32_t at = min(lane & 15, x.last) * 512 + (lane >> 4) * 16;
+  const uint32_t at = (WHOLE ? lane & 15 : min(lane & 15, x.last)) * 512 + (lane >> 4) * 16;
 #pragma unroll
   for (int j = 0; j < 4; ++j) k[j] = *reinterpret_cast<const uint4*>(x.at + 256 + 64 * j + at);
 }
+template <bool WHOLE>
 __device__ __forceinline__ void load_v(uint4 (&v)[4], const Tile& x, int lane) {
 #pragma unroll
-  for (int r = 0; r < 4; ++r)
-    v[r] = load_stream(x.at + (uint32_t)(min(4 * (lane >> 4) + r, x.last) * 512 + 16 * (lane & 15)));
+  for (int r = 0; r < 4; ++r) {
+    const int row = 4 * (lane >> 4) + r;
+    v[r] = load_stream(x.at + (uint32_t)((WHOLE ? row : min(row, x.last)) * 512 + 16 * (lane & 15)));
+  }
 }
 
 // ---------------------------------------------------------------- queries
@@ -208,22 +220,21 @@ __device__ __forceinline__ float tanh_near(float x) {
   return ax < 0.3f ? x * p : t;
 }
 
-// A score in log2 units from q . k: x in, with a cap x out tanh of that.
+// Scores in log2 units from q . k: x in; with a cap out tanh(x in).
 struct ScoreScale {
   float in, out;
   __device__ ScoreScale(float cap) {
     in = cap > 0.f ? 0.0625f / cap : 0.0625f * DN_LOG2E;
-    out = cap * DN_LOG2E;
+    out = cap > 0.f ? cap * DN_LOG2E : 1.f;
   }
-  template <bool CAP>
-  __device__ __forceinline__ float apply(float s) const {
-    if constexpr (CAP) return out * tanh_near(s * in);
-    return s * in;
-  }
-  // the same less a row's log total
-  template <bool CAP>
-  __device__ __forceinline__ float less(float s, float total) const {
-    return fmaf(CAP ? tanh_near(s * in) : s, CAP ? out : in, -total);
+  // of two tiles of 16 keys
+  __device__ __forceinline__ void apply(bool cap, const v4f (&s)[2], float (&z)[8]) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) z[e] = s[e >> 2][e & 3] * in;
+    if (cap) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) z[e] = out * tanh_near(z[e]);
+    }
   }
 };
 
@@ -249,28 +260,30 @@ __device__ __forceinline__ v2h fp8_f16x2(uint32_t w) {
   return __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.f, HI));
 }
 
-// Row operands of softmax x V for dims 16 c + 4 w + i of lane 16 kb + c: its 8
-// keys (4 kb + r of both tiles), transposed and widened.
+// Of a tile's V (lane 16 kb + c: dims 16 c .. +15 of keys 4 kb + r), dims 16 c +
+// 4 w + i of the 4 keys, transposed and widened: half i's 4 values.
+__device__ __forceinline__ void v_halves(const uint4 (&v)[4], int w, uint2 (&half)[4]) {
+  const uint32_t y[4] = {(&v[0].x)[w], (&v[1].x)[w], (&v[2].x)[w], (&v[3].x)[w]};
+  const uint32_t lo01 = __builtin_amdgcn_perm(y[1], y[0], 0x05010400u);
+  const uint32_t hi01 = __builtin_amdgcn_perm(y[1], y[0], 0x07030602u);
+  const uint32_t lo23 = __builtin_amdgcn_perm(y[3], y[2], 0x05010400u);
+  const uint32_t hi23 = __builtin_amdgcn_perm(y[3], y[2], 0x07030602u);
+  const uint32_t d[4] = {__builtin_amdgcn_perm(lo23, lo01, 0x05040100u), __builtin_amdgcn_perm(lo23, lo01, 0x07060302u),
+                         __builtin_amdgcn_perm(hi23, hi01, 0x05040100u), __builtin_amdgcn_perm(hi23, hi01, 0x07060302u)};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    half[i] = make_uint2(__builtin_bit_cast(uint32_t, fp8_f16x2<false>(d[i])),
+                         __builtin_bit_cast(uint32_t, fp8_f16x2<true>(d[i])));
+}
+
+// Row operands of softmax x V: element 4 x + r is key 4 kb + r of tile x.
 __device__ __forceinline__ void v_operands(const uint4 (&v)[2][4], int w, v8h (&va)[4]) {
-  uint32_t d[2][4];  // d[a][i]: the 4 keys' bytes of dim 4 w + i
+  uint2 half[2][4];
 #pragma unroll
-  for (int a = 0; a < 2; ++a) {
-    const uint32_t y[4] = {(&v[a][0].x)[w], (&v[a][1].x)[w], (&v[a][2].x)[w], (&v[a][3].x)[w]};
-    const uint32_t lo01 = __builtin_amdgcn_perm(y[1], y[0], 0x05010400u);
-    const uint32_t hi01 = __builtin_amdgcn_perm(y[1], y[0], 0x07030602u);
-    const uint32_t lo23 = __builtin_amdgcn_perm(y[3], y[2], 0x05010400u);
-    const uint32_t hi23 = __builtin_amdgcn_perm(y[3], y[2], 0x07030602u);
-    d[a][0] = __builtin_amdgcn_perm(lo23, lo01, 0x05040100u);
-    d[a][1] = __builtin_amdgcn_perm(lo23, lo01, 0x07060302u);
-    d[a][2] = __builtin_amdgcn_perm(hi23, hi01, 0x05040100u);
-    d[a][3] = __builtin_amdgcn_perm(hi23, hi01, 0x07060302u);
-  }
+  for (int x = 0; x < 2; ++x) v_halves(v[x], w, half[x]);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const v2h p[4] = {fp8_f16x2<false>(d[0][i]), fp8_f16x2<true>(d[0][i]),
-                      fp8_f16x2<false>(d[1][i]), fp8_f16x2<true>(d[1][i])};
-    va[i] = v8h{p[0][0], p[0][1], p[1][0], p[1][1], p[2][0], p[2][1], p[3][0], p[3][1]};
-  }
+  for (int i = 0; i < 4; ++i)
+    va[i] = __builtin_bit_cast(v8h, make_uint4(half[0][i].x, half[0][i].y, half[1][i].x, half[1][i].y));
 }
 
 // The partials: share k of sequence b has index k + b (each next one moves
@@ -294,58 +307,14 @@ struct Partials {
 };
 
 // ------------------------------------------------------------- attention
-// A block: KW waves along the keys x RW along the rows, RT tiles of 16 rows a
-// wave.  Registers: 64 RT sums, 32 of K, 32 of V a lane.
-template <int RT, int RW, int KW, bool CAP>
-__global__ __launch_bounds__(RW * KW * 64) void k_tree(TreeArgs a) {
-  constexpr int WAVES = RW * KW, TILES = RT * RW;
-  constexpr int JOIN = (KW / 2) * RW * RT * 16 * WAVE;  // float4: waves that hand over their sums
-  constexpr int IMG = TILES * IMG_TILE;
-  __shared__ uint4 s_buf[IMG > JOIN ? IMG : JOIN];  // the queries' image, then the sums in transit
-  __shared__ float2 s_ml[(KW / 2 + 1) * RW * RT * WAVE];
-  __shared__ uint64_t s_bits[TILES * 16];
-  __shared__ int s_start[CACHE_MAX_BATCH + 1];
-  __shared__ int s_nan;
-  const int g = blockIdx.y, k = blockIdx.x;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int rw = wave % RW, kw = wave / RW, col = lane & 15, kb = lane >> 4;
-  const Partials part(a.part, a.c.batch, a.n);
-  const int total = sequence_starts<false>(a.c, a.counts, a.n, s_start);
-  if (k == 0 && g == 0)
-    for (int b = threadIdx.x; b <= a.c.batch; b += WAVES * 64) part.starts[b] = s_start[b];
-  const int blocks = min((int)gridDim.x, total);
-  if (k >= blocks) return;
-  const int end = share_start(total, blocks, k + 1);
+// What a wave holds of RT tiles of 16 rows: lane (kb, col) sums of row col
+// (o[i][r]: dim 16 (4 kb + r) + i), the base of its exponents and its total.
+template <int RT>
+struct RowSums {
+  v4f o[RT][16];
+  float m[RT], l[RT];
 
-  for (int p0 = share_start(total, blocks, k); p0 < end;) {
-    const int b = sequence_of(s_start, a.c.batch, p0);
-    const int first = __builtin_amdgcn_readfirstlane(s_start[b]);
-    const int p1 = min(end, __builtin_amdgcn_readfirstlane(s_start[b + 1]));
-    const Sequence seq = Sequence(a.c, a.counts, a.n, b).uniform();
-    stage_queries<WAVES * 64>(a.q, b, g, TILES, seq.rows, s_buf);
-    for (int r = threadIdx.x; r < TILES * 16; r += WAVES * 64)
-      s_bits[r] = r < seq.rows ? row_mask(a.tree, a.n, b, r / H) : 0;
-    if (threadIdx.x == 0) s_nan = 0;
-    auto tiles = [&](int pair, Tile& x, Tile& y) {
-      const int t = (pair - first) * TR_PAIR;
-      x = tile_at(a.c, b, g, t, seq.keys);
-      y = tile_at(a.c, b, g, t + 16, seq.keys);
-    };
-    int j = p0 + kw;
-    uint4 kx[2][4], vx[2][4];
-    Tile t0, t1;
-    if (j < p1) {
-      tiles(j, t0, t1);
-      load_k(kx[0], t0, lane);
-      load_k(kx[1], t1, lane);
-      load_v(vx[0], t0, lane);
-      load_v(vx[1], t1, lane);
-    }
-    __syncthreads();
-
-    v4f o[RT][16];
-    float m[RT], l[RT];
-    const ScoreScale zs(a.cap);
+  __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
@@ -353,118 +322,51 @@ __global__ __launch_bounds__(RW * KW * 64) void k_tree(TreeArgs a) {
       m[rt] = -INFINITY;
       l[rt] = 0.f;
     }
-#pragma nounroll
-    for (; j < p1; j += KW) {
-      const int at = (j - first) * TR_PAIR;
-      const bool more = j + KW < p1;
-      const bool bad0 = t0.bad, bad1 = t1.bad;
-      // some of the keys are drafts, past the end or in no page
-      const bool edge = at + TR_PAIR > seq.len || bad0 || bad1;
-      if (more) tiles(j + KW, t0, t1);
-      float z[RT][8];
-      {
-        v4f acc[RT][2];
-        scores<RT>(kx, s_buf + rw * RT * IMG_TILE, lane, acc);
+  }
+
+  // Probabilities of 8 keys (log2 scores z, -inf: invisible) as column operand.
+  __device__ __forceinline__ v8h weigh(int rt, const float (&z)[8]) {
+    float tm = fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])), fmaxf(fmaxf(z[4], z[5]), fmaxf(z[6], z[7])));
+    if (__ballot(tm > m[rt] + TR_MOST)) {
+      tm = fmaxf(tm, __shfl_xor(tm, 16));
+      tm = fmaxf(tm, __shfl_xor(tm, 32));
+      const bool grow = tm > m[rt] + TR_MOST;
+      const float mn = grow ? tm - TR_BASE : m[rt];
+      const float al = grow ? __builtin_amdgcn_exp2f(m[rt] - mn) : 1.f;
+      l[rt] *= al;
+      m[rt] = mn;
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
+      for (int i = 0; i < 16; ++i)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) z[rt][e] = zs.template apply<CAP>(acc[rt][e >> 2][e & 3]);
-      }
-      // the scores are done before their records' registers are loaded anew
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) asm volatile("" : "+v"(z[rt][e]));
-      if (more) {
-        load_k(kx[0], t0, lane);
-        load_k(kx[1], t1, lane);
-      }
-      if (edge) {
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          const uint64_t bits = s_bits[(rw * RT + rt) * 16 + col];
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if ((e < 4 ? bad0 : bad1) || !sees(seq, bits, at + 16 * (e >> 2) + 4 * kb + (e & 3)))
-              z[rt][e] = -INFINITY;
-        }
-      }
-      v8h pb[RT];
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        float tm = z[rt][0];
-#pragma unroll
-        for (int e = 1; e < 8; ++e) tm = fmaxf(tm, z[rt][e]);
-        if (__ballot(tm > m[rt] + TR_MOST)) {
-          tm = fmaxf(tm, __shfl_xor(tm, 16));
-          tm = fmaxf(tm, __shfl_xor(tm, 32));
-          const bool grow = tm > m[rt] + TR_MOST;
-          const float mn = grow ? tm - TR_BASE : m[rt];
-          const float al = grow ? __builtin_amdgcn_exp2f(m[rt] - mn) : 1.f;
-          l[rt] *= al;
-          m[rt] = mn;
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) o[rt][i][r] *= al;
-        }
-        float p[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {  // (a masked key: 0, also while m = -inf)
-          const float x = __builtin_amdgcn_exp2f(z[rt][e] - m[rt]);
-          p[e] = z[rt][e] == -INFINITY ? 0.f : x;
-          pb[rt][e] = (_Float16)p[e];
-        }
-        l[rt] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-      }
-      if (edge) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if (bad0) vx[0][r] = make_uint4(0, 0, 0, 0);
-          if (bad1) vx[1][r] = make_uint4(0, 0, 0, 0);
-        }
-      }
-      if (at + TR_PAIR > seq.len) {
-        // 0 x NaN would reach the rows that do not see a draft with NaN in V:
-        // such a byte counts as 0 here, and the merge puts NaN where a row
-        // sees it
-        uint32_t any = 0;
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              uint32_t& v = (&vx[x][r].x)[w];
-              const uint32_t flag = nan_bytes(v) >> 7;
-              v &= ~(flag * 0xffu);
-              any |= flag;
-            }
-        if (__ballot(any != 0) && lane == 0) s_nan = 1;
-      }
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        v8h va[4];
-        v_operands(vx, w, va);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt)
-            o[rt][4 * w + i] =
-                __builtin_amdgcn_mfma_f32_16x16x32_f16(va[i], pb[rt], o[rt][4 * w + i], 0, 0, 0);
-        __builtin_amdgcn_sched_barrier(0);  // one word's operands live at a time
-      }
-      if (more) {
-        load_v(vx[0], t0, lane);
-        load_v(vx[1], t1, lane);
-      }
+        for (int r = 0; r < 4; ++r) o[rt][i][r] *= al;
     }
+    // while a row has seen nothing its m is -inf: 0 stands in, so that
+    // invisible keys give 2^-inf and not NaN
+    const float base = m[rt] == -INFINITY ? 0.f : m[rt];
+    float p[8];
+    v8h pb;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      p[e] = __builtin_amdgcn_exp2f(z[e] - base);
+      pb[e] = (_Float16)p[e];
+    }
+    l[rt] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+    return pb;
+  }
+
+  // Totals over the lanes of a row.
+  __device__ __forceinline__ void total() {
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       l[rt] += __shfl_xor(l[rt], 16);
       l[rt] += __shfl_xor(l[rt], 32);
     }
-    // the key waves' sums, halved in number by every step
+  }
+
+  // Joins the sums of the KW key waves of each row wave into kw 0, halving
+  // their number in every step.  buf: (KW / 2) RW RT 16 WAVE uint4.
+  template <int RW, int KW>
+  __device__ __forceinline__ void join(int rw, int kw, int lane, uint4* buf, float2* ml) {
 #pragma nounroll
     for (int live = KW; live > 1; live = (live + 1) / 2) {
       const int half = (live + 1) / 2;
@@ -475,8 +377,8 @@ __global__ __launch_bounds__(RW * KW * 64) void k_tree(TreeArgs a) {
         for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            s_buf[((slot * RT + rt) * 16 + i) * WAVE + lane] = __builtin_bit_cast(uint4, o[rt][i]);
-          s_ml[(slot * RT + rt) * WAVE + lane] = make_float2(m[rt], l[rt]);
+            buf[((slot * RT + rt) * 16 + i) * WAVE + lane] = __builtin_bit_cast(uint4, o[rt][i]);
+          ml[(slot * RT + rt) * WAVE + lane] = make_float2(m[rt], l[rt]);
         }
       }
       __syncthreads();
@@ -484,16 +386,16 @@ __global__ __launch_bounds__(RW * KW * 64) void k_tree(TreeArgs a) {
         const int slot = kw * RW + rw;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-          const float2 ml = s_ml[(slot * RT + rt) * WAVE + lane];
-          const float mn = fmaxf(m[rt], ml.x);
+          const float2 x = ml[(slot * RT + rt) * WAVE + lane];
+          const float mn = fmaxf(m[rt], x.x);
           // (an empty side counts 0: its m is -inf; a NaN total stays NaN)
           const float f0 = l[rt] == 0.f ? 0.f : __builtin_amdgcn_exp2f(m[rt] - mn);
-          const float f1 = ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - mn);
+          const float f1 = x.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(x.x - mn);
           m[rt] = mn;
-          l[rt] = fmaf(l[rt], f0, ml.y * f1);
+          l[rt] = fmaf(l[rt], f0, x.y * f1);
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const v4f other = __builtin_bit_cast(v4f, s_buf[((slot * RT + rt) * 16 + i) * WAVE + lane]);
+            const v4f other = __builtin_bit_cast(v4f, buf[((slot * RT + rt) * 16 + i) * WAVE + lane]);
 #pragma unroll
             for (int r = 0; r < 4; ++r) o[rt][i][r] = fmaf(o[rt][i][r], f0, other[r] * f1);
             if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // 4 loads in flight, not 16
@@ -501,26 +403,344 @@ __global__ __launch_bounds__(RW * KW * 64) void k_tree(TreeArgs a) {
         }
       }
     }
-    if (kw == 0) {
-      // o[i][r] of lane (kb, col) is dim 16 (4 kb + r) + i of row col
+  }
+
+  // Writes the partial of rows row0 .. (those below `rows`); at: its first row.
+  __device__ __forceinline__ void store(const Partials& part, size_t at, int row0, int rows, int lane) const {
+    const int col = lane & 15, kb = lane >> 4;
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        const int row = (rw * RT + rt) * 16 + col;
-        if (row >= seq.rows) continue;
-        const size_t at = g * part.rows + (size_t)(k + b) * a.n * H + row;
+    for (int rt = 0; rt < RT; ++rt) {
+      const int row = row0 + rt * 16 + col;
+      if (row >= rows) continue;
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+      for (int r = 0; r < 4; ++r)
 #pragma unroll
-          for (int i = 0; i < 16; i += 4)
-            *reinterpret_cast<float4*>(part.o + at * D + 16 * (4 * kb + r) + i) =
-                make_float4(o[rt][i][r], o[rt][i + 1][r], o[rt][i + 2][r], o[rt][i + 3][r]);
-        if (kb == 0) part.stats[at] = make_float2(m[rt], l[rt]);
+        for (int i = 0; i < 16; i += 4)
+          *reinterpret_cast<float4*>(part.o + (at + row) * D + 16 * (4 * kb + r) + i) =
+              make_float4(o[rt][i][r], o[rt][i + 1][r], o[rt][i + 2][r], o[rt][i + 3][r]);
+      if (kb == 0) part.stats[at + row] = make_float2(m[rt], l[rt]);
+    }
+  }
+};
+
+// The scores of invisible keys of a pair become -inf: of tiles without a page,
+// and with EDGE of drafts that the row does not see and keys past the end.
+template <bool EDGE>
+__device__ __forceinline__ void hide(float (&z)[8], const Sequence& seq, uint64_t bits, int at, int kb, bool bad0,
+                                     bool bad1) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const bool seen = !EDGE || sees(seq, bits, at + 16 * (e >> 2) + 4 * kb + (e & 3));
+    if ((e < 4 ? bad0 : bad1) || !seen) z[e] = -INFINITY;
+  }
+}
+
+// Takes NaN in 4 words as 0 (see k_tree_merge); whether there was one.
+__device__ __forceinline__ uint32_t drop_nan(uint4& v) {
+  uint32_t any = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    uint32_t& u = (&v.x)[w];
+    const uint32_t flag = nan_bytes(u) >> 7;
+    u &= ~(flag * 0xffu);
+    any |= flag;
+  }
+  return any;
+}
+
+// A block's share of the pairs of KV head g: the piece of one sequence after
+// the other, `piece` called for each.
+template <typename F>
+__device__ __forceinline__ void each_piece(const TreeArgs& a, const Partials& part, int* s_start, F piece) {
+  const int g = blockIdx.y, k = blockIdx.x;
+  const int total = sequence_starts<false>(a.c, a.counts, a.n, s_start);
+  if (k == 0 && g == 0)
+    for (int b = threadIdx.x; b <= a.c.batch; b += blockDim.x) part.starts[b] = s_start[b];
+  const int blocks = min((int)gridDim.x, total);
+  if (k >= blocks) return;
+  const int end = share_start(total, blocks, k + 1);
+  for (int p0 = share_start(total, blocks, k); p0 < end;) {
+    const int b = sequence_of(s_start, a.c.batch, p0);
+    const int first = __builtin_amdgcn_readfirstlane(s_start[b]);
+    const int p1 = min(end, __builtin_amdgcn_readfirstlane(s_start[b + 1]));
+    piece(b, first, p0, p1);
+    p0 = p1;
+  }
+}
+
+// A block: KW waves along the keys x RW along the rows, RT tiles of 16 rows a
+// wave; every wave loads its pairs of tiles itself, one pair in registers
+// whose K half is loaded anew after the scores and whose V half after the
+// sums.  Registers: 64 RT sums, 32 of K, 32 of V a lane.
+template <int RT, int RW, int KW, bool PAGED>
+__global__ __launch_bounds__(RW * KW * 64) void k_tree(TreeArgs a) {
+  constexpr int WAVES = RW * KW, TILES = RT * RW;
+  constexpr int JOIN = (KW / 2) * RW * RT * 16 * WAVE;
+  constexpr int IMG = TILES * IMG_TILE;
+  __shared__ uint4 s_buf[IMG > JOIN ? IMG : JOIN];  // the queries' image, then the sums in transit
+  __shared__ float2 s_ml[(KW / 2) * RW * RT * WAVE];
+  __shared__ uint64_t s_bits[TILES * 16];
+  __shared__ int s_start[CACHE_MAX_BATCH + 1];
+  __shared__ int s_nan;
+  const int g = blockIdx.y, k = blockIdx.x;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rw = wave % RW, kw = wave / RW, col = lane & 15, kb = lane >> 4;
+  const Partials part(a.part, a.c.batch, a.n);
+  const ScoreScale zs(a.cap);
+  const bool cap = a.cap > 0.f;
+  each_piece(a, part, s_start, [&](int b, int first, int p0, int p1) {
+    const Sequence seq = Sequence(a.c, a.counts, a.n, b).uniform();
+    const int whole = min(p1, first + seq.len / TR_PAIR);  // pairs of committed keys alone come first
+    stage_queries<WAVES * 64>(a.q, b, g, TILES, seq.rows, s_buf);
+    for (int r = threadIdx.x; r < TILES * 16; r += WAVES * 64)
+      s_bits[r] = r < seq.rows ? row_mask(a.tree, a.n, b, r / H) : 0;
+    if (threadIdx.x == 0) s_nan = 0;
+    Tile t[2];
+    uint4 kx[2][4], vx[2][4];
+    auto tiles = [&](int pair) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) t[x] = tile_at<PAGED>(a.c, b, g, (pair - first) * TR_PAIR + 16 * x, seq.keys);
+    };
+    int j = p0 + kw;
+    if (j < whole) {
+      tiles(j);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        load_k<true>(kx[x], t[x], lane);
+        load_v<true>(vx[x], t[x], lane);
       }
     }
-    p0 = p1;
+    __syncthreads();
+
+    RowSums<RT> sums;
+    sums.clear();
+    // one pair; EDGE: some of its keys are drafts or past the end (it loads
+    // its records itself)
+    auto step = [&](auto edge) {
+      constexpr bool EDGE = decltype(edge)::value;
+      const int at = (j - first) * TR_PAIR;
+      const bool more = !EDGE && j + KW < whole;
+      if (EDGE) {
+        tiles(j);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          load_k<false>(kx[x], t[x], lane);
+          load_v<false>(vx[x], t[x], lane);
+        }
+      }
+      const bool bad0 = t[0].bad, bad1 = t[1].bad;
+      if (more) tiles(j + KW);
+      v4f acc[RT][2];
+      scores<RT>(kx, s_buf + rw * RT * IMG_TILE, lane, acc);
+      // (done before their records' registers are loaded anew)
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) asm volatile("" : "+v"(acc[rt][x]));
+      if (more) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) load_k<true>(kx[x], t[x], lane);
+      }
+      v8h pb[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        float z[8];
+        zs.apply(cap, acc[rt], z);
+        if (EDGE || bad0 || bad1)
+          hide<EDGE>(z, seq, EDGE ? s_bits[(rw * RT + rt) * 16 + col] : 0, at, kb, bad0, bad1);
+        pb[rt] = sums.weigh(rt, z);
+      }
+      if (bad0 || bad1) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (bad0) vx[0][r] = make_uint4(0, 0, 0, 0);
+          if (bad1) vx[1][r] = make_uint4(0, 0, 0, 0);
+        }
+      }
+      if (EDGE) {
+        uint32_t any = 0;
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) any |= drop_nan(vx[x][r]);
+        if (__ballot(any != 0) && lane == 0) s_nan = 1;
+      }
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        v8h va[4];
+        v_operands(vx, w, va);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+            sums.o[rt][4 * w + i] =
+                __builtin_amdgcn_mfma_f32_16x16x32_f16(va[i], pb[rt], sums.o[rt][4 * w + i], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);  // one word's operands live at a time
+      }
+      if (more) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) load_v<true>(vx[x], t[x], lane);
+      }
+      j += KW;
+    };
+#pragma nounroll
+    while (j < whole) step(std::false_type{});
+#pragma nounroll
+    while (j < p1) step(std::true_type{});
+    sums.total();
+    sums.template join<RW, KW>(rw, kw, lane, s_buf, s_ml);
+    if (kw == 0)
+      sums.store(part, g * part.rows + (size_t)(k + b) * a.n * H, rw * RT * 16, seq.rows, lane);
     __syncthreads();  // the buffer is formed anew
     if (threadIdx.x == 0) part.nan[g * part.shares + k + b] = s_nan;
-  }
+  });
+}
+
+// More than 16 drafts (64 rows): as many row waves would each widen the same
+// records.  Here the block's 8 waves load and widen two pairs together into
+// LDS, twice buffered, and every wave reads its operands there; the queries
+// stay in registers.  RW row waves of 32 rows, KW = 8 / RW key waves.
+template <int RW, bool PAGED>
+__global__ __launch_bounds__(512) void k_tree_wide(TreeArgs a) {
+  constexpr int RT = 2, KW = 8 / RW, TILES = RT * RW;
+  constexpr int KBUF = 2 * 2 * IMG_TILE;   // uint4: [pair][tile][step][lane]
+  constexpr int VBUF = 2 * 16 * WAVE;      // uint4: [pair][dim of 16][lane], tile x in half x
+  constexpr int BUF = KBUF + VBUF;         // 64 KB
+  __shared__ uint4 s_buf[2 * BUF];
+  __shared__ float2 s_ml[(KW / 2 + 1) * RW * RT * WAVE];
+  __shared__ uint64_t s_bits[TILES * 16];
+  __shared__ int s_bad[2][4];
+  __shared__ int s_start[CACHE_MAX_BATCH + 1];
+  __shared__ int s_nan;
+  static_assert((KW / 2) * RW * RT * 16 * WAVE <= 2 * BUF, "the sums in transit fit");
+  const int g = blockIdx.y, k = blockIdx.x;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rw = wave % RW, kw = wave / RW, col = lane & 15, kb = lane >> 4;
+  // what the wave loads: tile sx of pair sp, K or V (each SIMD has one of both)
+  const int sx = wave & 1, sp = (wave >> 1) & 1;
+  const bool sv = wave >= 4;
+  const Partials part(a.part, a.c.batch, a.n);
+  const ScoreScale zs(a.cap);
+  const bool cap = a.cap > 0.f;
+  each_piece(a, part, s_start, [&](int b, int first, int p0, int p1) {
+    const Sequence seq = Sequence(a.c, a.counts, a.n, b).uniform();
+    for (int r = threadIdx.x; r < TILES * 16; r += 512)
+      s_bits[r] = r < seq.rows ? row_mask(a.tree, a.n, b, r / H) : 0;
+    if (threadIdx.x == 0) s_nan = 0;
+    v8bf q[RT][STEPS];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int row = (rw * RT + rt) * 16 + col;
+      const bool real = row < seq.rows;
+      const uint16_t* src = static_cast<const uint16_t*>(a.q.data) + b * a.q.sb +
+                            (real ? row / H : 0) * a.q.st + (g * H + row % H) * a.q.sh;
+#pragma unroll
+      for (int step = 0; step < STEPS; ++step)
+        q[rt][step] = __builtin_bit_cast(v8bf, *reinterpret_cast<const uint4*>(src + step_dim(step, kb)));
+    }
+    const int steps = (p1 - p0 + 1) / 2;
+    uint4 in[4];
+    Tile t;
+    auto load = [&](int it) {  // (past the last pair: its last tile again, not used)
+      const int pair = min(p0 + 2 * it + sp, p1 - 1);
+      t = tile_at<PAGED>(a.c, b, g, (pair - first) * TR_PAIR + 16 * sx, seq.keys);
+      if (sv) load_v<false>(in, t, lane);
+      else load_k<false>(in, t, lane);
+    };
+    auto widen = [&](int it) {
+      uint4* buf = s_buf + (it & 1) * BUF;
+      const int pair = min(p0 + 2 * it + sp, p1 - 1);
+      if (sv) {
+        if (PAGED && t.bad) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) in[r] = make_uint4(0, 0, 0, 0);
+        }
+        if ((pair - first + 1) * TR_PAIR > seq.len) {
+          uint32_t any = 0;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) any |= drop_nan(in[r]);
+          if (__ballot(any != 0) && lane == 0) s_nan = 1;
+        }
+        uint2* out = reinterpret_cast<uint2*>(buf + KBUF + sp * 16 * WAVE + lane) + sx;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint2 half[4];
+          v_halves(in, w, half);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) out[(4 * w + i) * WAVE * 2] = half[i];
+        }
+      } else {
+        uint4* out = buf + (sp * 2 + sx) * IMG_TILE + lane;
+#pragma unroll
+        for (int step = 0; step < STEPS; ++step) {
+          const uint4 w = in[step >> 1];
+          out[step * WAVE] = __builtin_bit_cast(uint4, (step & 1) ? k_operand(w.z, w.w) : k_operand(w.x, w.y));
+        }
+        if (lane == 0) s_bad[it & 1][sp * 2 + sx] = t.bad;
+      }
+    };
+    load(0);
+    widen(0);
+    if (steps > 1) load(1);
+    __syncthreads();
+
+    RowSums<RT> sums;
+    sums.clear();
+#pragma nounroll
+    for (int it = 0; it < steps; ++it) {
+      const uint4* buf = s_buf + (it & 1) * BUF;
+#pragma nounroll
+      for (int pair = kw; pair < 2; pair += KW) {
+        const int j = p0 + 2 * it + pair;
+        if (j >= p1) break;
+        const int at = (j - first) * TR_PAIR;
+        v4f acc[RT][2];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) acc[rt][0] = acc[rt][1] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int step = 0; step < STEPS; ++step)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const v8bf kk = __builtin_bit_cast(v8bf, buf[((pair * 2 + x) * STEPS + step) * WAVE + lane]);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+              acc[rt][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kk, q[rt][step], acc[rt][x], 0, 0, 0);
+          }
+        const bool edge = at + TR_PAIR > seq.len;
+        bool bad0 = false, bad1 = false;
+        if constexpr (PAGED) {
+          bad0 = __builtin_amdgcn_readfirstlane(s_bad[it & 1][pair * 2]) != 0;
+          bad1 = __builtin_amdgcn_readfirstlane(s_bad[it & 1][pair * 2 + 1]) != 0;
+        }
+        v8h pb[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          float z[8];
+          zs.apply(cap, acc[rt], z);
+          if (edge) hide<true>(z, seq, s_bits[(rw * RT + rt) * 16 + col], at, kb, bad0, bad1);
+          else if (bad0 || bad1) hide<false>(z, seq, 0, at, kb, bad0, bad1);
+          pb[rt] = sums.weigh(rt, z);
+        }
+        const uint4* vb = buf + KBUF + pair * 16 * WAVE + lane;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const v8h va = __builtin_bit_cast(v8h, vb[i * WAVE]);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+            sums.o[rt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb[rt], sums.o[rt][i], 0, 0, 0);
+        }
+      }
+      if (it + 1 < steps) widen(it + 1);
+      if (it + 2 < steps) load(it + 2);
+      __syncthreads();
+    }
+    sums.total();
+    sums.template join<RW, KW>(rw, kw, lane, s_buf, s_ml);
+    if (kw == 0)
+      sums.store(part, g * part.rows + (size_t)(k + b) * a.n * H, rw * RT * 16, seq.rows, lane);
+    __syncthreads();
+    if (threadIdx.x == 0) part.nan[g * part.shares + k + b] = s_nan;
+  });
 }
 
 // Row (b, g, row) = blockIdx.x, dims 64 blockIdx.y + [0, 64): thread (slice,
@@ -601,7 +821,7 @@ __global__ __launch_bounds__(256) void k_tree_merge(TreeArgs a, int shares) {
 // rows in registers and then over the 16 lanes of a row group.
 constexpr int KWT_WAVES = 8;
 
-template <int TILES, bool CAP>
+template <int TILES, bool PAGED>
 __global__ __launch_bounds__(KWT_WAVES * 64) void k_key_weights(WeightArgs a) {
   __shared__ uint4 s_img[TILES * IMG_TILE];
   __shared__ float s_lse[TILES * 16];
@@ -611,6 +831,7 @@ __global__ __launch_bounds__(KWT_WAVES * 64) void k_key_weights(WeightArgs a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, kb = lane >> 4;
   const ScoreScale zs(a.cap);
+  const bool cap = a.cap > 0.f;
   const int total = sequence_starts<true>(a.c, a.counts, a.n, s_start);
   const int blocks = min((int)gridDim.x, total);
   if (k >= blocks) return;
@@ -625,13 +846,13 @@ __global__ __launch_bounds__(KWT_WAVES * 64) void k_key_weights(WeightArgs a) {
     int j = p0 + wave;
     auto tiles = [&](int pair, Tile& x, Tile& y) {
       const int t = (pair - first) * TR_PAIR;
-      x = tile_at(a.c, b, g, t, seq.keys);
-      y = tile_at(a.c, b, g, t + 16, seq.keys);
+      x = tile_at<PAGED>(a.c, b, g, t, seq.keys);
+      y = tile_at<PAGED>(a.c, b, g, t + 16, seq.keys);
     };
     if (j < p1) {
       tiles(j, t0, t1);
-      load_k(kx[0], t0, lane);
-      load_k(kx[1], t1, lane);
+      load_k<false>(kx[0], t0, lane);
+      load_k<false>(kx[1], t1, lane);
     }
     stage_queries<KWT_WAVES * 64>(a.q, b, g, TILES, seq.rows, s_img);
     for (int r = threadIdx.x; r < TILES * 16; r += KWT_WAVES * 64) {
@@ -659,8 +880,8 @@ __global__ __launch_bounds__(KWT_WAVES * 64) void k_key_weights(WeightArgs a) {
         }
       if (j + KWT_WAVES < p1) {
         tiles(j + KWT_WAVES, t0, t1);
-        load_k(kx[0], t0, lane);
-        load_k(kx[1], t1, lane);
+        load_k<false>(kx[0], t0, lane);
+        load_k<false>(kx[1], t1, lane);
       }
       float sum[8];
 #pragma unroll
@@ -677,9 +898,11 @@ __global__ __launch_bounds__(KWT_WAVES * 64) void k_key_weights(WeightArgs a) {
           for (int x = 0; x < 2; ++x)
             acc[x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka[x][step], q, acc[x], 0, 0, 0);
         }
+        float z[8];
+        zs.apply(cap, acc, z);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          float p = __builtin_amdgcn_exp2f(zs.template less<CAP>(acc[e >> 2][e & 3], lse));
+          float p = __builtin_amdgcn_exp2f(z[e] - lse);
           if (edge) {
             const bool seen = !(e < 4 ? bad0 : bad1) &&
                               sees(seq, s_bits[row], at + 16 * (e >> 2) + 4 * kb + (e & 3));
@@ -709,27 +932,27 @@ __global__ __launch_bounds__(KWT_WAVES * 64) void k_key_weights(WeightArgs a) {
   }
 }
 
-template <bool CAP>
+template <bool PAGED>
 void tree_rows(const TreeArgs& a, hipStream_t st) {
   const dim3 grid(TR_BLOCKS, G);
   const int tiles = (a.n * H + 15) / 16;
-  if (tiles <= 1) hipLaunchKernelGGL((k_tree<1, 1, 12, CAP>), grid, dim3(768), 0, st, a);
-  else if (tiles <= 2) hipLaunchKernelGGL((k_tree<2, 1, 8, CAP>), grid, dim3(512), 0, st, a);
-  else if (tiles <= 4) hipLaunchKernelGGL((k_tree<2, 2, 4, CAP>), grid, dim3(512), 0, st, a);
-  else if (tiles <= 8) hipLaunchKernelGGL((k_tree<2, 4, 2, CAP>), grid, dim3(512), 0, st, a);
-  else hipLaunchKernelGGL((k_tree<2, 8, 1, CAP>), grid, dim3(512), 0, st, a);
+  if (tiles <= 1) hipLaunchKernelGGL((k_tree<1, 1, 12, PAGED>), grid, dim3(768), 0, st, a);
+  else if (tiles <= 2) hipLaunchKernelGGL((k_tree<2, 1, 8, PAGED>), grid, dim3(512), 0, st, a);
+  else if (tiles <= 4) hipLaunchKernelGGL((k_tree<2, 2, 4, PAGED>), grid, dim3(512), 0, st, a);
+  else if (tiles <= 8) hipLaunchKernelGGL((k_tree_wide<4, PAGED>), grid, dim3(512), 0, st, a);
+  else hipLaunchKernelGGL((k_tree_wide<8, PAGED>), grid, dim3(512), 0, st, a);
 }
 
-template <bool CAP>
+template <bool PAGED>
 void weight_rows(const WeightArgs& a, hipStream_t st) {
   const int tiles = (a.n * H + 15) / 16;
   const dim3 block(KWT_WAVES * 64);
   const dim3 grid(tiles <= 8 ? 2 * TR_BLOCKS : TR_BLOCKS, G);
-  if (tiles <= 1) hipLaunchKernelGGL((k_key_weights<1, CAP>), grid, block, 0, st, a);
-  else if (tiles <= 2) hipLaunchKernelGGL((k_key_weights<2, CAP>), grid, block, 0, st, a);
-  else if (tiles <= 4) hipLaunchKernelGGL((k_key_weights<4, CAP>), grid, block, 0, st, a);
-  else if (tiles <= 8) hipLaunchKernelGGL((k_key_weights<8, CAP>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((k_key_weights<16, CAP>), grid, block, 0, st, a);
+  if (tiles <= 1) hipLaunchKernelGGL((k_key_weights<1, PAGED>), grid, block, 0, st, a);
+  else if (tiles <= 2) hipLaunchKernelGGL((k_key_weights<2, PAGED>), grid, block, 0, st, a);
+  else if (tiles <= 4) hipLaunchKernelGGL((k_key_weights<4, PAGED>), grid, block, 0, st, a);
+  else if (tiles <= 8) hipLaunchKernelGGL((k_key_weights<8, PAGED>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((k_key_weights<16, PAGED>), grid, block, 0, st, a);
 }
 
 }  // namespace
@@ -740,13 +963,13 @@ size_t tree_workspace(int batch, int n) {
 }
 
 void launch_tree(const TreeArgs& a, hipStream_t st) {
-  (a.cap > 0.f ? tree_rows<true> : tree_rows<false>)(a, st);
+  (a.c.table ? tree_rows<true> : tree_rows<false>)(a, st);
   hipLaunchKernelGGL(k_tree_merge, dim3((unsigned)(a.c.batch * G * a.n * H), D / 64), dim3(256), 0, st,
                      a, TR_BLOCKS);
 }
 
 void launch_key_weights(const WeightArgs& a, hipStream_t st) {
-  (a.cap > 0.f ? weight_rows<true> : weight_rows<false>)(a, st);
+  (a.c.table ? weight_rows<true> : weight_rows<false>)(a, st);
 }
 
 }  // namespace skv
