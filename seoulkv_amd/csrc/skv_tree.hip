@@ -59,19 +59,20 @@ struct Sequence {
   }
 };
 
-// s_start[b]: pairs of the sequences before b; s_start[batch]: all.  With
-// WHOLE a sequence without rows counts too.
+// Pairs of a sequence; with WHOLE one without rows counts too.
+template <bool WHOLE>
+__device__ __forceinline__ int sequence_pairs(const Sequence& s) {
+  return WHOLE || s.rows ? (s.keys + TR_PAIR - 1) / TR_PAIR : 0;
+}
+
+// s_start[b]: pairs of the sequences before b; s_start[batch]: all.
 template <bool WHOLE>
 __device__ __forceinline__ int sequence_starts(const CacheView& c, const int* counts, int n, int* s_start) {
   if (threadIdx.x < WAVE) {
     int carry = 0;
     for (int b0 = 0; b0 < c.batch; b0 += WAVE) {
       const int b = b0 + threadIdx.x;
-      int pairs = 0;
-      if (b < c.batch) {
-        const Sequence s(c, counts, n, b);
-        if (WHOLE || s.rows) pairs = (s.keys + TR_PAIR - 1) / TR_PAIR;
-      }
+      const int pairs = b < c.batch ? sequence_pairs<WHOLE>(Sequence(c, counts, n, b)) : 0;
       const int inc = wave_incl_scan(pairs);
       if (b < c.batch) s_start[b] = carry + inc - pairs;
       carry += __builtin_amdgcn_readlane(inc, WAVE - 1);
@@ -211,29 +212,40 @@ __device__ __forceinline__ void scores(const uint4 (&k)[2][4], const uint4* img,
   }
 }
 
-// tanh to about an ulp: a polynomial near 0, where 1 - 2 / (e^2x + 1) cancels.
-__device__ __forceinline__ float tanh_near(float x) {
-  const float ax = fabsf(x), x2 = x * x;
-  const float e = __builtin_amdgcn_exp2f(ax * (2.f * DN_LOG2E));
-  const float t = copysignf(fmaf(-2.f, __builtin_amdgcn_rcpf(e + 1.f), 1.f), x);
-  const float p = fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
-  return ax < 0.3f ? x * p : t;
-}
-
-// Scores in log2 units from q . k: x in; with a cap out tanh(x in).
+// Scores in log2 units are s unit; s is q . k, or with a cap q . k put through
+// cap tanh(x / cap) in units of q . k, x = q . k / 16.
 struct ScoreScale {
-  float in, out;
-  __device__ ScoreScale(float cap) {
-    in = cap > 0.f ? 0.0625f / cap : 0.0625f * DN_LOG2E;
-    out = cap > 0.f ? cap * DN_LOG2E : 1.f;
+  float unit;
+  float in, out;  // x / cap = in q . k; cap in units of q . k
+  __device__ explicit ScoreScale(float cap) {
+    unit = 0.0625f * DN_LOG2E;
+    in = cap > 0.f ? 0.0625f / cap : 0.f;
+    out = 16.f * cap;
   }
-  // of two tiles of 16 keys
-  __device__ __forceinline__ void apply(bool cap, const v4f (&s)[2], float (&z)[8]) const {
+  // Caps the scores of two tiles of 16 keys.  Up to half the cap 7 terms of the
+  // series are exact to 9e-8; where all of a wave's scores are, as is usual,
+  // the exponential and the reciprocal are not needed.
+  __device__ __forceinline__ void squash(v4f (&s)[2]) const {
+    // tanh(in s) = in s (1 + c[0] s^2 + c[1] s^4 + ..)
+    constexpr float T[6] = {-1.f / 3.f, 2.f / 15.f, -17.f / 315.f, 62.f / 2835.f, -1382.f / 155925.f,
+                            21844.f / 6081075.f};
+    float c[6], power = 1.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) z[e] = s[e >> 2][e & 3] * in;
-    if (cap) {
+    for (int i = 0; i < 6; ++i) c[i] = T[i] * (power *= in * in);
+    float most = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) z[e] = out * tanh_near(z[e]);
+    for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(s[e >> 2][e & 3]));
+    const bool near = __ballot(!(most * in < 0.5f)) == 0;  // (NaN: passed on either way)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = s[e >> 2][e & 3], u = x * x;
+      const float p = x * fmaf(u, fmaf(u, fmaf(u, fmaf(u, fmaf(u, fmaf(u, c[5], c[4]), c[3]), c[2]), c[1]), c[0]), 1.f);
+      s[e >> 2][e & 3] = p;
+      if (!near) {
+        const float ax = fabsf(x * in);
+        const float far = fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(ax * (2.f * DN_LOG2E)) + 1.f), 1.f);
+        s[e >> 2][e & 3] = ax < 0.5f ? p : copysignf(out * far, x);
+      }
     }
   }
 };
@@ -287,23 +299,27 @@ __device__ __forceinline__ void v_operands(const uint4 (&v)[2][4], int w, v8h (&
 }
 
 // The partials: share k of sequence b has index k + b (each next one moves
-// either k or b on by one).  [G][blocks + batch][rows][256] sums, then as many
-// (m, total) pairs, then [G][blocks + batch] flags (see k_tree_merge), then
-// the sequences' starts.
+// either k or b on by one).  [G][blocks + batch][tiles] of 16 rows as the waves
+// hold them, [16 i][lane] four sums (RowSums) and [16] (m, total) pairs: whole
+// lines both ways.  Then [G][blocks + batch] flags (see k_tree_merge), then the
+// sequences' starts.
 struct Partials {
-  float* o;
+  float4* o;
   float2* stats;
   int* nan;
   int* starts;
-  size_t rows, shares;  // per group
-  __host__ __device__ Partials(float* part, int batch, int n) {
+  size_t shares;  // per group
+  int tiles;
+  __host__ __device__ Partials(void* part, int batch, int n) {
     shares = TR_BLOCKS + batch;
-    rows = shares * n * H;
-    o = part;
-    stats = reinterpret_cast<float2*>(o + rows * G * D);
-    nan = reinterpret_cast<int*>(stats + rows * G);
+    tiles = (n * H + 15) / 16;
+    o = static_cast<float4*>(part);
+    stats = reinterpret_cast<float2*>(o + shares * G * tiles * 16 * WAVE);
+    nan = reinterpret_cast<int*>(stats + shares * G * tiles * 16);
     starts = nan + shares * G;
   }
+  // Tile 0 of share k of sequence b.
+  __device__ __forceinline__ size_t tile(int g, int k, int b) const { return (g * shares + k + b) * tiles; }
 };
 
 // ------------------------------------------------------------- attention
@@ -324,9 +340,11 @@ struct RowSums {
     }
   }
 
-  // Probabilities of 8 keys (log2 scores z, -inf: invisible) as column operand.
-  __device__ __forceinline__ v8h weigh(int rt, const float (&z)[8]) {
-    float tm = fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])), fmaxf(fmaxf(z[4], z[5]), fmaxf(z[6], z[7])));
+  // Probabilities of 8 keys from their scores s (-inf: invisible; s unit: in
+  // log2 units) as column operand.
+  __device__ __forceinline__ v8h weigh(int rt, const v4f (&s)[2], float unit) {
+    float tm = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                     fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3]))) * unit;
     if (__ballot(tm > m[rt] + TR_MOST)) {
       tm = fmaxf(tm, __shfl_xor(tm, 16));
       tm = fmaxf(tm, __shfl_xor(tm, 32));
@@ -347,7 +365,7 @@ struct RowSums {
     v8h pb;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      p[e] = __builtin_amdgcn_exp2f(z[e] - base);
+      p[e] = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][e & 3], unit, -base));
       pb[e] = (_Float16)p[e];
     }
     l[rt] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
@@ -363,18 +381,21 @@ struct RowSums {
     }
   }
 
-  // Joins the sums of the KW key waves of each row wave into kw 0, halving
-  // their number in every step.  buf: (KW / 2) RW RT 16 WAVE uint4.
-  template <int RW, int KW>
-  __device__ __forceinline__ void join(int rw, int kw, int lane, uint4* buf, float2* ml) {
+  // Joins the sums of the first `live` key waves of each row wave into kw 0,
+  // halving their number in every step; `rows`: the real ones (the others'
+  // lanes move nothing).  buf: (live / 2) RW RT 16 WAVE uint4.
+  template <int RW>
+  __device__ __forceinline__ void join(int live, int rw, int kw, int rows, int lane, uint4* buf, float2* ml) {
+    const int row = rw * RT * 16 + (lane & 15);
 #pragma nounroll
-    for (int live = KW; live > 1; live = (live + 1) / 2) {
+    for (; live > 1; live = (live + 1) / 2) {
       const int half = (live + 1) / 2;
       __syncthreads();
       if (kw >= half && kw < live) {
         const int slot = (kw - half) * RW + rw;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
+          if (row + rt * 16 >= rows) continue;
 #pragma unroll
           for (int i = 0; i < 16; ++i)
             buf[((slot * RT + rt) * 16 + i) * WAVE + lane] = __builtin_bit_cast(uint4, o[rt][i]);
@@ -386,6 +407,7 @@ struct RowSums {
         const int slot = kw * RW + rw;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
+          if (row + rt * 16 >= rows) continue;
           const float2 x = ml[(slot * RT + rt) * WAVE + lane];
           const float mn = fmaxf(m[rt], x.x);
           // (an empty side counts 0: its m is -inf; a NaN total stays NaN)
@@ -405,20 +427,16 @@ struct RowSums {
     }
   }
 
-  // Writes the partial of rows row0 .. (those below `rows`); at: its first row.
-  __device__ __forceinline__ void store(const Partials& part, size_t at, int row0, int rows, int lane) const {
-    const int col = lane & 15, kb = lane >> 4;
+  // Writes the partial of tiles tile0 .., of which rows below `rows` are real.
+  __device__ __forceinline__ void store(const Partials& part, size_t tile, int tile0, int rows, int lane) const {
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      const int row = row0 + rt * 16 + col;
-      if (row >= rows) continue;
+      if ((tile0 + rt) * 16 + (lane & 15) >= rows) continue;
+      const size_t at = tile + tile0 + rt;
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int i = 0; i < 16; i += 4)
-          *reinterpret_cast<float4*>(part.o + (at + row) * D + 16 * (4 * kb + r) + i) =
-              make_float4(o[rt][i][r], o[rt][i + 1][r], o[rt][i + 2][r], o[rt][i + 3][r]);
-      if (kb == 0) part.stats[at + row] = make_float2(m[rt], l[rt]);
+      for (int i = 0; i < 16; ++i)
+        part.o[(at * 16 + i) * WAVE + lane] = make_float4(o[rt][i][0], o[rt][i][1], o[rt][i][2], o[rt][i][3]);
+      if (lane < 16) part.stats[at * 16 + lane] = make_float2(m[rt], l[rt]);
     }
   }
 };
@@ -426,12 +444,12 @@ struct RowSums {
 // The scores of invisible keys of a pair become -inf: of tiles without a page,
 // and with EDGE of drafts that the row does not see and keys past the end.
 template <bool EDGE>
-__device__ __forceinline__ void hide(float (&z)[8], const Sequence& seq, uint64_t bits, int at, int kb, bool bad0,
+__device__ __forceinline__ void hide(v4f (&s)[2], const Sequence& seq, uint64_t bits, int at, int kb, bool bad0,
                                      bool bad1) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const bool seen = !EDGE || sees(seq, bits, at + 16 * (e >> 2) + 4 * kb + (e & 3));
-    if ((e < 4 ? bad0 : bad1) || !seen) z[e] = -INFINITY;
+    if ((e < 4 ? bad0 : bad1) || !seen) s[e >> 2][e & 3] = -INFINITY;
   }
 }
 
@@ -449,20 +467,31 @@ __device__ __forceinline__ uint32_t drop_nan(uint4& v) {
 }
 
 // A block's share of the pairs of KV head g: the piece of one sequence after
-// the other, `piece` called for each.
+// the other, `piece` called for each.  A single sequence (the latency of short
+// contexts) needs no starts.
 template <typename F>
-__device__ __forceinline__ void each_piece(const TreeArgs& a, const Partials& part, int* s_start, F piece) {
+__device__ __forceinline__ void each_piece(const TreeArgs& a, int* s_start, F piece) {
   const int g = blockIdx.y, k = blockIdx.x;
-  const int total = sequence_starts<false>(a.c, a.counts, a.n, s_start);
-  if (k == 0 && g == 0)
-    for (int b = threadIdx.x; b <= a.c.batch; b += blockDim.x) part.starts[b] = s_start[b];
+  int total;
+  if (a.c.batch == 1) {
+    total = sequence_pairs<false>(Sequence(a.c, a.counts, a.n, 0).uniform());
+  } else {
+    total = sequence_starts<false>(a.c, a.counts, a.n, s_start);
+    if (k == 0 && g == 0) {
+      int* starts = Partials(a.part, a.c.batch, a.n).starts;
+      for (int b = threadIdx.x; b <= a.c.batch; b += blockDim.x) starts[b] = s_start[b];
+    }
+  }
   const int blocks = min((int)gridDim.x, total);
   if (k >= blocks) return;
   const int end = share_start(total, blocks, k + 1);
   for (int p0 = share_start(total, blocks, k); p0 < end;) {
-    const int b = sequence_of(s_start, a.c.batch, p0);
-    const int first = __builtin_amdgcn_readfirstlane(s_start[b]);
-    const int p1 = min(end, __builtin_amdgcn_readfirstlane(s_start[b + 1]));
+    int b = 0, first = 0, p1 = end;
+    if (a.c.batch > 1) {
+      b = sequence_of(s_start, a.c.batch, p0);
+      first = __builtin_amdgcn_readfirstlane(s_start[b]);
+      p1 = min(end, __builtin_amdgcn_readfirstlane(s_start[b + 1]));
+    }
     piece(b, first, p0, p1);
     p0 = p1;
   }
@@ -485,10 +514,15 @@ __global__ __launch_bounds__(RW * KW * 64) void k_tree(TreeArgs a) {
   const int g = blockIdx.y, k = blockIdx.x;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rw = wave % RW, kw = wave / RW, col = lane & 15, kb = lane >> 4;
-  const Partials part(a.part, a.c.batch, a.n);
+  // (formed where it is used: its addresses do not stay in registers)
+  auto partials = [&] {
+    float* at = a.part;
+    asm volatile("" : "+s"(at));
+    return Partials(at, a.c.batch, a.n);
+  };
   const ScoreScale zs(a.cap);
   const bool cap = a.cap > 0.f;
-  each_piece(a, part, s_start, [&](int b, int first, int p0, int p1) {
+  each_piece(a, s_start, [&](int b, int first, int p0, int p1) {
     const Sequence seq = Sequence(a.c, a.counts, a.n, b).uniform();
     const int whole = min(p1, first + seq.len / TR_PAIR);  // pairs of committed keys alone come first
     stage_queries<WAVES * 64>(a.q, b, g, TILES, seq.rows, s_buf);
@@ -544,11 +578,10 @@ __global__ __launch_bounds__(RW * KW * 64) void k_tree(TreeArgs a) {
       v8h pb[RT];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        float z[8];
-        zs.apply(cap, acc[rt], z);
+        if (cap) zs.squash(acc[rt]);
         if (EDGE || bad0 || bad1)
-          hide<EDGE>(z, seq, EDGE ? s_bits[(rw * RT + rt) * 16 + col] : 0, at, kb, bad0, bad1);
-        pb[rt] = sums.weigh(rt, z);
+          hide<EDGE>(acc[rt], seq, EDGE ? s_bits[(rw * RT + rt) * 16 + col] : 0, at, kb, bad0, bad1);
+        pb[rt] = sums.weigh(rt, acc[rt], zs.unit);
       }
       if (bad0 || bad1) {
 #pragma unroll
@@ -588,41 +621,45 @@ __global__ __launch_bounds__(RW * KW * 64) void k_tree(TreeArgs a) {
 #pragma nounroll
     while (j < p1) step(std::true_type{});
     sums.total();
-    sums.template join<RW, KW>(rw, kw, lane, s_buf, s_ml);
+    sums.template join<RW>(min(KW, p1 - p0), rw, kw, seq.rows, lane, s_buf, s_ml);  // (waves without a pair hold nothing)
+    const Partials part = partials();
     if (kw == 0)
-      sums.store(part, g * part.rows + (size_t)(k + b) * a.n * H, rw * RT * 16, seq.rows, lane);
+      sums.store(part, part.tile(g, k, b), rw * RT, seq.rows, lane);
     __syncthreads();  // the buffer is formed anew
     if (threadIdx.x == 0) part.nan[g * part.shares + k + b] = s_nan;
   });
 }
 
-// More than 16 drafts (64 rows): as many row waves would each widen the same
-// records.  Here the block's 8 waves load and widen two pairs together into
-// LDS, twice buffered, and every wave reads its operands there; the queries
-// stay in registers.  RW row waves of 32 rows, KW = 8 / RW key waves.
-template <int RW, bool PAGED>
+// More than 32 drafts: 8 row waves of 32 rows would each widen the same
+// records.  Here they load and widen two pairs together into LDS, twice
+// buffered, and every wave reads its operands there; the queries stay in
+// registers.
+template <bool PAGED>
 __global__ __launch_bounds__(512) void k_tree_wide(TreeArgs a) {
-  constexpr int RT = 2, KW = 8 / RW, TILES = RT * RW;
+  constexpr int RT = 2, TILES = 16;
   constexpr int KBUF = 2 * 2 * IMG_TILE;   // uint4: [pair][tile][step][lane]
   constexpr int VBUF = 2 * 16 * WAVE;      // uint4: [pair][dim of 16][lane], tile x in half x
   constexpr int BUF = KBUF + VBUF;         // 64 KB
   __shared__ uint4 s_buf[2 * BUF];
-  __shared__ float2 s_ml[(KW / 2 + 1) * RW * RT * WAVE];
   __shared__ uint64_t s_bits[TILES * 16];
   __shared__ int s_bad[2][4];
   __shared__ int s_start[CACHE_MAX_BATCH + 1];
   __shared__ int s_nan;
-  static_assert((KW / 2) * RW * RT * 16 * WAVE <= 2 * BUF, "the sums in transit fit");
   const int g = blockIdx.y, k = blockIdx.x;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int rw = wave % RW, kw = wave / RW, col = lane & 15, kb = lane >> 4;
+  const int col = lane & 15, kb = lane >> 4;
   // what the wave loads: tile sx of pair sp, K or V (each SIMD has one of both)
   const int sx = wave & 1, sp = (wave >> 1) & 1;
   const bool sv = wave >= 4;
-  const Partials part(a.part, a.c.batch, a.n);
+  // (formed where it is used: its addresses do not stay in registers)
+  auto partials = [&] {
+    float* at = a.part;
+    asm volatile("" : "+s"(at));
+    return Partials(at, a.c.batch, a.n);
+  };
   const ScoreScale zs(a.cap);
   const bool cap = a.cap > 0.f;
-  each_piece(a, part, s_start, [&](int b, int first, int p0, int p1) {
+  each_piece(a, s_start, [&](int b, int first, int p0, int p1) {
     const Sequence seq = Sequence(a.c, a.counts, a.n, b).uniform();
     for (int r = threadIdx.x; r < TILES * 16; r += 512)
       s_bits[r] = r < seq.rows ? row_mask(a.tree, a.n, b, r / H) : 0;
@@ -630,7 +667,7 @@ __global__ __launch_bounds__(512) void k_tree_wide(TreeArgs a) {
     v8bf q[RT][STEPS];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      const int row = (rw * RT + rt) * 16 + col;
+      const int row = (wave * RT + rt) * 16 + col;
       const bool real = row < seq.rows;
       const uint16_t* src = static_cast<const uint16_t*>(a.q.data) + b * a.q.sb +
                             (real ? row / H : 0) * a.q.st + (g * H + row % H) * a.q.sh;
@@ -686,11 +723,12 @@ __global__ __launch_bounds__(512) void k_tree_wide(TreeArgs a) {
 
     RowSums<RT> sums;
     sums.clear();
+    if (wave >= 4) __builtin_amdgcn_s_setprio(1);  // the two waves of a SIMD drift apart: one multiplies, one weighs
 #pragma nounroll
     for (int it = 0; it < steps; ++it) {
       const uint4* buf = s_buf + (it & 1) * BUF;
 #pragma nounroll
-      for (int pair = kw; pair < 2; pair += KW) {
+      for (int pair = 0; pair < 2; ++pair) {
         const int j = p0 + 2 * it + pair;
         if (j >= p1) break;
         const int at = (j - first) * TR_PAIR;
@@ -715,11 +753,10 @@ __global__ __launch_bounds__(512) void k_tree_wide(TreeArgs a) {
         v8h pb[RT];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-          float z[8];
-          zs.apply(cap, acc[rt], z);
-          if (edge) hide<true>(z, seq, s_bits[(rw * RT + rt) * 16 + col], at, kb, bad0, bad1);
-          else if (bad0 || bad1) hide<false>(z, seq, 0, at, kb, bad0, bad1);
-          pb[rt] = sums.weigh(rt, z);
+          if (cap) zs.squash(acc[rt]);
+          if (edge) hide<true>(acc[rt], seq, s_bits[(wave * RT + rt) * 16 + col], at, kb, bad0, bad1);
+          else if (bad0 || bad1) hide<false>(acc[rt], seq, 0, at, kb, bad0, bad1);
+          pb[rt] = sums.weigh(rt, acc[rt], zs.unit);
         }
         const uint4* vb = buf + KBUF + pair * 16 * WAVE + lane;
 #pragma unroll
@@ -735,83 +772,138 @@ __global__ __launch_bounds__(512) void k_tree_wide(TreeArgs a) {
       __syncthreads();
     }
     sums.total();
-    sums.template join<RW, KW>(rw, kw, lane, s_buf, s_ml);
-    if (kw == 0)
-      sums.store(part, g * part.rows + (size_t)(k + b) * a.n * H, rw * RT * 16, seq.rows, lane);
+    const Partials part = partials();
+    sums.store(part, part.tile(g, k, b), wave * RT, seq.rows, lane);
     __syncthreads();
     if (threadIdx.x == 0) part.nan[g * part.shares + k + b] = s_nan;
   });
 }
 
-// Row (b, g, row) = blockIdx.x, dims 64 blockIdx.y + [0, 64): thread (slice,
-// 4 dims) adds partials slice, slice + 16, ...; the slices are added in order.
+// Joins the partials of a tile of rows, NI of the 16 sums i at a time (unit =
+// (b, g, tile, i / NI)).  SLICES waves each add every SLICES-th share and the
+// slices are added in order: 8 for few sequences, which have up to 64 shares
+// each, with NI 1 where there are few rows too, so that all of a wave's shares
+// are in flight at once; 1 (4 units a block) for many rows with few shares.
 // Where a share met NaN in V among the last keys (it took them as 0), those
 // keys are gone through once more and the dims in which the row sees one
 // become NaN.
-__global__ __launch_bounds__(256) void k_tree_merge(TreeArgs a, int shares) {
-  const int R = a.n * H;
-  const int row = blockIdx.x % R, g = (blockIdx.x / R) % G, b = blockIdx.x / (R * G);
-  const int dl = threadIdx.x & 15, sl = threadIdx.x >> 4, d = blockIdx.y * 64 + 4 * dl;
-  __shared__ float4 s_o[16][16];
-  __shared__ float s_m[16], s_l[16];
+template <int SLICES, int NI>
+__global__ __launch_bounds__(SLICES == 1 ? 256 : SLICES * 64) void k_tree_merge(TreeArgs a, int shares) {
+  constexpr int PER = 16 / NI;  // units of a tile
   const Partials part(a.part, a.c.batch, a.n);
-  const int i = row / H, head = g * H + row % H;
-  const size_t at = ((size_t)b * a.n + i) * G * H + head;
-  const int total = part.starts[a.c.batch], start = part.starts[b], stop = part.starts[b + 1];
-  const Sequence seq(a.c, a.counts, a.n, b);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int unit = SLICES == 1 ? blockIdx.x * 4 + wave : blockIdx.x, sl = SLICES == 1 ? 0 : wave;
+  const int i0 = unit % PER * NI, tile = unit / PER % part.tiles, g = unit / PER / part.tiles % G,
+            b = unit / (PER * part.tiles * G);
+  __shared__ float4 s_o[SLICES == 1 ? 1 : SLICES][NI][WAVE];
+  __shared__ float2 s_ml[SLICES == 1 ? 1 : SLICES][16];
+  const Sequence seq = Sequence(a.c, a.counts, a.n, b).uniform();
+  int total, start = 0;
+  int stop = total = sequence_pairs<false>(seq);
+  if (a.c.batch > 1) {
+    total = part.starts[a.c.batch];
+    start = part.starts[b];
+    stop = part.starts[b + 1];
+  }
   float m = -INFINITY, l = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  v4f o[NI];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) o[i] = v4f{0.f, 0.f, 0.f, 0.f};
   int nan = 0;
+  // the factors of what is held and of one more share
+  auto join = [&](float2 ml, float& f0, float& f1) {
+    const float mn = fmaxf(m, ml.x);
+    f0 = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+    f1 = ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - mn);
+    m = mn;
+    l = fmaf(l, f0, ml.y * f1);
+  };
+  const int row = tile * 16 + (lane & 15);
   if (row < seq.rows && start < stop) {
     const int blocks = min(shares, total);
     const int k1 = share_of(total, blocks, stop - 1);
-    for (int k = share_of(total, blocks, start) + sl; k <= k1; k += 16) {
-      const size_t from = g * part.rows + (size_t)(k + b) * R + row;
-      nan |= part.nan[g * part.shares + k + b];
-      const float2 ml = part.stats[from];
-      const float4 x = *reinterpret_cast<const float4*>(part.o + from * D + d);
-      const float mn = fmaxf(m, ml.x);
-      const float f0 = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-      const float f1 = ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - mn);
-      m = mn;
-      l = fmaf(l, f0, ml.y * f1);
-      o.x = fmaf(o.x, f0, x.x * f1);
-      o.y = fmaf(o.y, f0, x.y * f1);
-      o.z = fmaf(o.z, f0, x.z * f1);
-      o.w = fmaf(o.w, f0, x.w * f1);
+    constexpr int U = NI == 1 ? 8 : 4;  // shares in flight
+    for (int k = share_of(total, blocks, start) + sl; k <= k1; k += U * SLICES) {
+      float2 ml[U];
+      float4 x[U][NI];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int ku = min(k + u * SLICES, k1);
+        const size_t at = part.tile(g, ku, b) + tile;
+        ml[u] = part.stats[at * 16 + (lane & 15)];
+        if (k + u * SLICES > k1) ml[u] = make_float2(-INFINITY, 0.f);  // (none left: adds nothing)
+        nan |= part.nan[g * part.shares + ku + b];
+#pragma unroll
+        for (int i = 0; i < NI; ++i) x[u][i] = part.o[(at * 16 + i0 + i) * WAVE + lane];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float f0, f1;
+        join(ml[u], f0, f1);
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const float v[4] = {x[u][i].x, x[u][i].y, x[u][i].z, x[u][i].w};
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[i][r] = fmaf(o[i][r], f0, v[r] * f1);
+        }
+      }
     }
   }
-  s_o[sl][dl] = o;
-  if (dl == 0) {
-    s_m[sl] = m;
-    s_l[sl] = l;
-  }
-  nan = __syncthreads_or(nan);
-  if (threadIdx.x < 64) {
-    float M = -INFINITY, L = 0.f, O = 0.f;
+  // dims 64 kb + 16 r + i0 + [0, NI) of the row, for r = r0 .. r1 - 1
+  int r0 = 0, r1 = 4;
+  if constexpr (SLICES > 1) {
 #pragma unroll
-    for (int s = 0; s < 16; ++s) M = fmaxf(M, s_m[s]);
+    for (int i = 0; i < NI; ++i) s_o[sl][i][lane] = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
+    if (lane < 16) s_ml[sl][lane] = make_float2(m, l);
+    nan = __syncthreads_or(nan);
+    if (sl >= 4) return;  // wave r < 4 finishes its dims
+    r0 = sl;
+    r1 = sl + 1;
+    m = -INFINITY;
+    l = 0.f;
+    float sum[NI];
 #pragma unroll
-    for (int s = 0; s < 16; ++s) {
-      const float f = s_l[s] == 0.f ? 0.f : __builtin_amdgcn_exp2f(s_m[s] - M);
-      L = fmaf(s_l[s], f, L);
-      O = fmaf((&s_o[s][threadIdx.x >> 2].x)[threadIdx.x & 3], f, O);
+    for (int i = 0; i < NI; ++i) sum[i] = 0.f;
+#pragma unroll
+    for (int s = 0; s < SLICES; ++s) {
+      float f0, f1;
+      join(s_ml[s][lane & 15], f0, f1);
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+        sum[i] = fmaf(sum[i], f0, reinterpret_cast<const float*>(&s_o[s][i][lane])[sl] * f1);
     }
-    const int dim = blockIdx.y * 64 + threadIdx.x;
-    float y = L == 0.f ? 0.f : O / L;
-    if (nan) {
-      const uint64_t bits = row_mask(a.tree, a.n, b, i);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) o[i] = v4f{sum[i], sum[i], sum[i], sum[i]};
+  }
+  if (row >= a.n * H) return;
+  const size_t at = ((size_t)b * a.n + row / H) * G * H + g * H + row % H;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    if (r < r0 || r >= r1) continue;
+    const int dim = 64 * (lane >> 4) + 16 * r + i0;
+    float y[NI];
+#pragma unroll
+    for (int i = 0; i < NI; ++i) y[i] = l == 0.f ? 0.f : o[i][r] * inv;
+    if (nan && row < seq.rows) {
+      const uint64_t bits = row_mask(a.tree, a.n, b, row / H);
       for (int t = seq.len & ~(TR_PAIR - 1); t < seq.keys; ++t) {
         const uint32_t page = a.c.table ? a.c.page(b, t) : 0;
         if (!sees(seq, bits, t) || (a.c.table && page >= a.c.n_pages)) continue;
         const size_t record = a.c.table ? a.c.row_in(page, g, t) : a.c.row(b, g, t);
-        if ((a.c.records[record * 512 + dim] & 0x7f) == 0x7f) y = __builtin_nanf("");
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+          if ((a.c.records[record * 512 + dim + i] & 0x7f) == 0x7f) y[i] = __builtin_nanf("");
       }
     }
-    a.out[at * D + dim] = (uint16_t)bf16_rne(y);
-    if (blockIdx.y == 0 && threadIdx.x == 0)
-      a.lse[at] = L == 0.f ? -INFINITY : (M + __log2f(L)) * TR_LN2;
+    uint16_t* out = a.out + at * D + dim;
+    if constexpr (NI == 4)
+      *reinterpret_cast<uint2*>(out) =
+          make_uint2(bf16_rne(y[0]) | bf16_rne(y[1]) << 16, bf16_rne(y[2]) | bf16_rne(y[3]) << 16);
+    else
+      out[0] = (uint16_t)bf16_rne(y[0]);
   }
+  if (i0 == 0 && r0 == 0 && lane < 16) a.lse[at] = l == 0.f ? -INFINITY : (m + __log2f(l)) * TR_LN2;
 }
 
 // ------------------------------------------------------------ key weights
@@ -819,10 +911,12 @@ __global__ __launch_bounds__(256) void k_tree_merge(TreeArgs a, int shares) {
 // stride the share, each with all rows of its 32 keys: the queries' image is
 // in LDS, the K halves in registers, and a key's weight is summed over the
 // rows in registers and then over the 16 lanes of a row group.
-constexpr int KWT_WAVES = 8;
+// (the 128 KB image of 64 drafts leaves room for one block, of 16 waves then)
+constexpr int weight_waves(int tiles) { return tiles > 8 ? 16 : 8; }
 
 template <int TILES, bool PAGED>
-__global__ __launch_bounds__(KWT_WAVES * 64) void k_key_weights(WeightArgs a) {
+__global__ __launch_bounds__(weight_waves(TILES) * 64, 4) void k_key_weights(WeightArgs a) {
+  constexpr int WAVES = weight_waves(TILES);
   __shared__ uint4 s_img[TILES * IMG_TILE];
   __shared__ float s_lse[TILES * 16];
   __shared__ uint64_t s_bits[TILES * 16];
@@ -832,14 +926,18 @@ __global__ __launch_bounds__(KWT_WAVES * 64) void k_key_weights(WeightArgs a) {
   const int col = lane & 15, kb = lane >> 4;
   const ScoreScale zs(a.cap);
   const bool cap = a.cap > 0.f;
-  const int total = sequence_starts<true>(a.c, a.counts, a.n, s_start);
+  const int total = a.c.batch == 1 ? sequence_pairs<true>(Sequence(a.c, a.counts, a.n, 0).uniform())
+                                   : sequence_starts<true>(a.c, a.counts, a.n, s_start);
   const int blocks = min((int)gridDim.x, total);
   if (k >= blocks) return;
   const int end = share_start(total, blocks, k + 1);
   for (int p0 = share_start(total, blocks, k); p0 < end;) {
-    const int b = sequence_of(s_start, a.c.batch, p0);
-    const int first = __builtin_amdgcn_readfirstlane(s_start[b]);
-    const int p1 = min(end, __builtin_amdgcn_readfirstlane(s_start[b + 1]));
+    int b = 0, first = 0, p1 = end;
+    if (a.c.batch > 1) {
+      b = sequence_of(s_start, a.c.batch, p0);
+      first = __builtin_amdgcn_readfirstlane(s_start[b]);
+      p1 = min(end, __builtin_amdgcn_readfirstlane(s_start[b + 1]));
+    }
     const Sequence seq = Sequence(a.c, a.counts, a.n, b).uniform();
     uint4 kx[2][4];
     Tile t0, t1;
@@ -849,13 +947,8 @@ __global__ __launch_bounds__(KWT_WAVES * 64) void k_key_weights(WeightArgs a) {
       x = tile_at<PAGED>(a.c, b, g, t, seq.keys);
       y = tile_at<PAGED>(a.c, b, g, t + 16, seq.keys);
     };
-    if (j < p1) {
-      tiles(j, t0, t1);
-      load_k<false>(kx[0], t0, lane);
-      load_k<false>(kx[1], t1, lane);
-    }
-    stage_queries<KWT_WAVES * 64>(a.q, b, g, TILES, seq.rows, s_img);
-    for (int r = threadIdx.x; r < TILES * 16; r += KWT_WAVES * 64) {
+    stage_queries<WAVES * 64>(a.q, b, g, TILES, seq.rows, s_img);
+    for (int r = threadIdx.x; r < TILES * 16; r += WAVES * 64) {
       const int i = r / H;
       const bool row = r < seq.rows;
       s_bits[r] = row ? row_mask(a.tree, a.n, b, i) : 0;
@@ -865,8 +958,12 @@ __global__ __launch_bounds__(KWT_WAVES * 64) void k_key_weights(WeightArgs a) {
     __syncthreads();
     const int used = (seq.rows + 15) / 16;
 #pragma nounroll
-    for (; j < p1; j += KWT_WAVES) {
+    for (; j < p1; j += WAVES) {
       const int at = (j - first) * TR_PAIR;
+      // nothing is loaded ahead: with 4 waves on a SIMD the others compute
+      tiles(j, t0, t1);
+      load_k<false>(kx[0], t0, lane);
+      load_k<false>(kx[1], t1, lane);
       const bool bad0 = t0.bad, bad1 = t1.bad;
       const bool edge = at + TR_PAIR > seq.len || bad0 || bad1;
       // widened once for all rows; the records' registers are loaded anew
@@ -878,11 +975,6 @@ __global__ __launch_bounds__(KWT_WAVES * 64) void k_key_weights(WeightArgs a) {
           const uint4 w = kx[x][step >> 1];
           ka[x][step] = (step & 1) ? k_operand(w.z, w.w) : k_operand(w.x, w.y);
         }
-      if (j + KWT_WAVES < p1) {
-        tiles(j + KWT_WAVES, t0, t1);
-        load_k<false>(kx[0], t0, lane);
-        load_k<false>(kx[1], t1, lane);
-      }
       float sum[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) sum[e] = 0.f;
@@ -898,11 +990,10 @@ __global__ __launch_bounds__(KWT_WAVES * 64) void k_key_weights(WeightArgs a) {
           for (int x = 0; x < 2; ++x)
             acc[x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka[x][step], q, acc[x], 0, 0, 0);
         }
-        float z[8];
-        zs.apply(cap, acc, z);
+        if (cap) zs.squash(acc);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          float p = __builtin_amdgcn_exp2f(z[e] - lse);
+          float p = __builtin_amdgcn_exp2f(fmaf(acc[e >> 2][e & 3], zs.unit, -lse));
           if (edge) {
             const bool seen = !(e < 4 ? bad0 : bad1) &&
                               sees(seq, s_bits[row], at + 16 * (e >> 2) + 4 * kb + (e & 3));
@@ -936,17 +1027,17 @@ template <bool PAGED>
 void tree_rows(const TreeArgs& a, hipStream_t st) {
   const dim3 grid(TR_BLOCKS, G);
   const int tiles = (a.n * H + 15) / 16;
-  if (tiles <= 1) hipLaunchKernelGGL((k_tree<1, 1, 12, PAGED>), grid, dim3(768), 0, st, a);
+  if (tiles <= 1) hipLaunchKernelGGL((k_tree<1, 1, 8, PAGED>), grid, dim3(512), 0, st, a);
   else if (tiles <= 2) hipLaunchKernelGGL((k_tree<2, 1, 8, PAGED>), grid, dim3(512), 0, st, a);
   else if (tiles <= 4) hipLaunchKernelGGL((k_tree<2, 2, 4, PAGED>), grid, dim3(512), 0, st, a);
-  else if (tiles <= 8) hipLaunchKernelGGL((k_tree_wide<4, PAGED>), grid, dim3(512), 0, st, a);
-  else hipLaunchKernelGGL((k_tree_wide<8, PAGED>), grid, dim3(512), 0, st, a);
+  else if (tiles <= 8) hipLaunchKernelGGL((k_tree<2, 4, 2, PAGED>), grid, dim3(512), 0, st, a);
+  else hipLaunchKernelGGL(k_tree_wide<PAGED>, grid, dim3(512), 0, st, a);
 }
 
 template <bool PAGED>
 void weight_rows(const WeightArgs& a, hipStream_t st) {
   const int tiles = (a.n * H + 15) / 16;
-  const dim3 block(KWT_WAVES * 64);
+  const dim3 block(weight_waves(tiles) * 64);
   const dim3 grid(tiles <= 8 ? 2 * TR_BLOCKS : TR_BLOCKS, G);
   if (tiles <= 1) hipLaunchKernelGGL((k_key_weights<1, PAGED>), grid, block, 0, st, a);
   else if (tiles <= 2) hipLaunchKernelGGL((k_key_weights<2, PAGED>), grid, block, 0, st, a);
@@ -964,8 +1055,15 @@ size_t tree_workspace(int batch, int n) {
 
 void launch_tree(const TreeArgs& a, hipStream_t st) {
   (a.c.table ? tree_rows<true> : tree_rows<false>)(a, st);
-  hipLaunchKernelGGL(k_tree_merge, dim3((unsigned)(a.c.batch * G * a.n * H), D / 64), dim3(256), 0, st,
-                     a, TR_BLOCKS);
+  const int tiles = a.c.batch * G * ((a.n * H + 15) / 16);
+  if (tiles <= 16)
+    hipLaunchKernelGGL((k_tree_merge<8, 1>), dim3(tiles * 16), dim3(512), 0, st, a, TR_BLOCKS);
+  else if (a.c.batch <= 4)
+    hipLaunchKernelGGL((k_tree_merge<8, 4>), dim3(tiles * 4), dim3(512), 0, st, a, TR_BLOCKS);
+  else if (a.c.batch <= 16)
+    hipLaunchKernelGGL((k_tree_merge<4, 4>), dim3(tiles * 4), dim3(256), 0, st, a, TR_BLOCKS);
+  else
+    hipLaunchKernelGGL((k_tree_merge<1, 4>), dim3(tiles), dim3(256), 0, st, a, TR_BLOCKS);
 }
 
 void launch_key_weights(const WeightArgs& a, hipStream_t st) {
