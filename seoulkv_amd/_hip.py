@@ -108,6 +108,7 @@ TRACE_LIB_PATH = LIB_PATH.with_name("libseoulkv4_hip_trace.so")
 
 _lib = None
 _trace_lib = None
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def load_library() -> ctypes.CDLL:
@@ -140,6 +141,7 @@ def load_trace_library() -> ctypes.CDLL | None:
 
 def _bind(lib: ctypes.CDLL) -> ctypes.CDLL:
     vp, i32, i64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64
+    cache, rows, turns = (ctypes.POINTER(t) for t in (RecordCacheDesc, RowsDesc, RotaryDesc))
     sig = {
         "skv_create": (i32, [ctypes.POINTER(IndexDesc), vp, vp, i32, vp, ctypes.POINTER(vp)]),
         "skv_create_paged": (i32, [ctypes.POINTER(IndexDesc), vp, vp, ctypes.POINTER(KVPagesDesc),
@@ -164,12 +166,12 @@ def _bind(lib: ctypes.CDLL) -> ctypes.CDLL:
         "skv_append_device": (i32, [vp, vp, vp, i32]),
         "skv_dense_decode": (i32, [vp]),
         "skv_dense_decode_static": (i32, [vp, i32, i32, vp, vp, vp]),
-        "skv_rotary": (i32, [vp, vp, vp, i32, i32, i32, i32, i32, vp, i64, i32, i32, vp]),
-        "skv_cache_write": (i32, [vp, vp, vp, vp, vp, vp, i32, vp, i32, vp, vp]),
-        "skv_tree_decode": (i32, [vp, vp, i32, vp, vp, ctypes.c_float, vp, vp, vp, i64, vp]),
+        "skv_rotary": (i32, [turns, rows, rows, i32, i32, i32, i32, i32, vp, i64, i32, i32, vp]),
+        "skv_cache_write": (i32, [cache, turns, rows, rows, rows, rows, i32, vp, i32, vp, vp]),
+        "skv_tree_decode": (i32, [cache, rows, i32, vp, vp, ctypes.c_float, vp, vp, vp, i64, vp]),
         "skv_tree_workspace": (i64, [i32, i32]),
-        "skv_key_weights": (i32, [vp, vp, i32, vp, vp, vp, ctypes.c_float, i32, vp]),
-        "skv_evict": (i32, [vp, vp, i32, i32, i32, vp, i64, vp]),
+        "skv_key_weights": (i32, [cache, rows, i32, vp, vp, vp, ctypes.c_float, i32, vp]),
+        "skv_evict": (i32, [cache, cache, i32, i32, i32, vp, i64, vp]),
         "skv_evict_workspace": (i64, [i32, i32, i32]),
         "skv_dense_output_device": (i32, [vp, ctypes.POINTER(vp)]),
         "skv_read_dense_output": (i32, [vp, vp]),
@@ -222,33 +224,21 @@ def dense_decode_static(kv8: torch.Tensor, context: int, q: torch.Tensor,
         raise RuntimeError(f"skv_dense_decode_static failed ({ERRORS.get(code, code)}): {msg}")
 
 
-class on_device:
-    """``with on_device(dev) as stream``: ``dev`` is the current device and
-    ``stream`` PyTorch's current stream there, for a call without a handle."""
-
-    __slots__ = ("index", "_guard")
-
-    def __init__(self, device: torch.device):
-        self.index = torch.cuda.current_device() if device.index is None else device.index
-        self._guard = None
-
-    def __enter__(self):
-        if torch.cuda.current_device() != self.index:
-            self._guard = torch.cuda.device(self.index)
-            self._guard.__enter__()
-        return torch.cuda.current_stream(self.index).cuda_stream or None
-
-    def __exit__(self, *exc):
-        if self._guard is not None:
-            self._guard.__exit__(*exc)
-
-
-def check_call(what: str, code: int) -> None:
-    """Raise for a failed call without a handle: ``ValueError`` for arguments
-    it refused, ``RuntimeError`` for anything else."""
+def call_on(device: int, name: str, *args) -> None:
+    """Call a library function without a handle, ``device`` its current device
+    and PyTorch's current stream there its last argument.  Raises
+    ``ValueError`` for arguments it refused, ``RuntimeError`` for anything
+    else."""
+    lib = _lib or load_library()
+    stream = _raw_stream(device)  # torch.cuda.current_stream(device).cuda_stream, 1 us sooner
+    if torch.cuda.current_device() == device:
+        code = getattr(lib, name)(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            code = getattr(lib, name)(*args, stream)
     if code != 0:
-        msg = load_library().skv_last_error(None).decode()
-        raise (ValueError if code == 1 else RuntimeError)(f"{what} failed ({ERRORS.get(code, code)}): {msg}")
+        msg = lib.skv_last_error(None).decode()
+        raise (ValueError if code == 1 else RuntimeError)(f"{name} failed ({ERRORS.get(code, code)}): {msg}")
 
 
 def pointer(t: torch.Tensor | None) -> int | None:

@@ -32,8 +32,6 @@ Calls may overlap (other streams) unless one writes what another reads.
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from seoulkv_amd import _hip
@@ -73,6 +71,7 @@ class RecordCache:
             raise ValueError("expected contiguous records [batch, 4, capacity, 512] or pages "
                              "[n_pages, 4, page_tokens, 512]")
         self._pool, self.records, self.device = pool, records, records.device
+        self._index = records.device.index
         self._owned: list[int] = []
         self.shared = False
         if page_table is None:
@@ -173,23 +172,25 @@ class RecordCache:
     def _open(self):
         if self._desc is None:
             raise RuntimeError("RecordCache is closed")
-        return ctypes.byref(self._desc)
+        return self._desc
 
     def _writable(self):
         if self.shared:
             raise ValueError("sequences of this cache share pages: it can only be read")
 
     def _rows(self, name, t, heads):
-        if not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16 or t.device != self.device \
-                or t.dim() != 4 or t.shape[0] != self.batch or tuple(t.shape[2:]) != (heads, HEAD_DIM):
+        """A BF16 tensor [batch, n, heads, 256] on this device, its last
+        dimension contiguous."""
+        shape = t.shape if isinstance(t, torch.Tensor) else ()
+        if len(shape) != 4 or shape[0] != self.batch or shape[2] != heads or shape[3] != HEAD_DIM \
+                or t.dtype != torch.bfloat16 or t.device != self.device:
             raise ValueError(f"expected BF16 {name} [{self.batch}, n, {heads}, {HEAD_DIM}] on {self.device}")
         return t if t.stride(3) == 1 else t.contiguous()
 
     def _optional(self, name, t, dtypes, shape):
         if t is None:
             return None
-        if not isinstance(t, torch.Tensor) or t.dtype not in dtypes or tuple(t.shape) != shape \
-                or t.device != self.device:
+        if not isinstance(t, torch.Tensor) or t.dtype not in dtypes or t.shape != shape or t.device != self.device:
             raise ValueError(f"expected {name} {list(shape)} of {' or '.join(map(str, dtypes))} on {self.device}")
         return t.contiguous()
 
@@ -197,7 +198,8 @@ class RecordCache:
         q = self._rows("q", q, N_HEADS)
         if q.shape[1] > MAX_DRAFTS:
             raise ValueError(f"{q.shape[1]} drafts above {MAX_DRAFTS}")
-        if q.data_ptr() % 16 or any(s % 8 for s in q.stride()[:3]):
+        b, n, h, _ = q.stride()
+        if q.data_ptr() % 16 or (b | n | h) % 8:
             q = q.clone(memory_format=torch.contiguous_format)  # 16-byte rows
         return q
 
@@ -228,7 +230,7 @@ class RecordCache:
             if q.shape[1] != n:
                 raise ValueError("q and k hold different numbers of tokens")
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+                q_out = q.new_empty(q.shape)
             elif q_out.stride(-1) != 1 or self._rows("q_out", q_out, N_HEADS).shape != q.shape:
                 raise ValueError("q_out must be like q, its last dimension contiguous")
         elif q_out is not None:
@@ -241,14 +243,10 @@ class RecordCache:
         _no_grad("write", k, v, q)
         if n == 0:
             return q_out
-        with _hip.on_device(self.device) as stream:
-            _hip.check_call("skv_cache_write", _hip.load_library().skv_cache_write(
-                desc, None if table is None else ctypes.byref(table._desc),
-                ctypes.byref(_hip.rows_desc(k)), ctypes.byref(_hip.rows_desc(v)),
-                None if q is None else ctypes.byref(_hip.rows_desc(q)),
-                None if q is None else ctypes.byref(_hip.rows_desc(q_out)),
-                n, _hip.pointer(positions),
-                int(positions is not None and positions.dtype == torch.int64), _hip.pointer(counts), stream))
+        _hip.call_on(self._index, "skv_cache_write", desc, None if table is None else table._desc,
+                     _hip.rows_desc(k), _hip.rows_desc(v), None if q is None else _hip.rows_desc(q),
+                     None if q is None else _hip.rows_desc(q_out), n, _hip.pointer(positions),
+                     positions is not None and positions.dtype == torch.int64, _hip.pointer(counts))
         return q_out
 
     def tree_decode(self, q: torch.Tensor, tree: torch.Tensor | None = None, *,
@@ -270,22 +268,19 @@ class RecordCache:
         counts = self._optional("counts", counts, (torch.int32,), (self.batch,))
         _no_grad("tree_decode", q)
         if out is None:
-            out = torch.empty((self.batch, n, N_HEADS, HEAD_DIM), dtype=q.dtype, device=self.device)
+            out = q.new_empty((self.batch, n, N_HEADS, HEAD_DIM))
         elif not out.is_contiguous() or self._rows("out", out, N_HEADS).shape[1] != n:
             raise ValueError("out must be contiguous and like q")
         if lse is None:
-            lse = torch.empty((self.batch, n, N_HEADS), device=self.device)
+            lse = q.new_empty((self.batch, n, N_HEADS), dtype=torch.float32)
         else:
             self._kept("lse", lse, torch.float32, (self.batch, n, N_HEADS))
         if n == 0:
             return out, lse
-        lib = _hip.load_library()
-        with _hip.on_device(self.device) as stream:
-            size = lib.skv_tree_workspace(self.batch, n)
-            work = torch.empty(size, dtype=torch.uint8, device=self.device)
-            _hip.check_call("skv_tree_decode", lib.skv_tree_decode(
-                desc, ctypes.byref(_hip.rows_desc(q)), n, _hip.pointer(tree), _hip.pointer(counts),
-                float(cap), out.data_ptr(), lse.data_ptr(), work.data_ptr(), size, stream))
+        size = _hip.load_library().skv_tree_workspace(self.batch, n)
+        work = q.new_empty(size, dtype=torch.uint8)
+        _hip.call_on(self._index, "skv_tree_decode", desc, _hip.rows_desc(q), n, _hip.pointer(tree),
+                     _hip.pointer(counts), cap, out.data_ptr(), lse.data_ptr(), work.data_ptr(), size)
         return out, lse
 
     def key_weights(self, q: torch.Tensor, lse: torch.Tensor, tree: torch.Tensor | None = None, *,
@@ -307,10 +302,8 @@ class RecordCache:
         _no_grad("key_weights", q, lse)
         if n == 0:
             raise ValueError("key_weights needs at least one row")
-        with _hip.on_device(self.device) as stream:
-            _hip.check_call("skv_key_weights", _hip.load_library().skv_key_weights(
-                desc, ctypes.byref(_hip.rows_desc(q)), n, lse.data_ptr(), _hip.pointer(tree),
-                _hip.pointer(counts), float(cap), int(bool(accumulate)), stream))
+        _hip.call_on(self._index, "skv_key_weights", desc, _hip.rows_desc(q), n, lse.data_ptr(),
+                     _hip.pointer(tree), _hip.pointer(counts), cap, bool(accumulate))
 
     def evict(self, to: "RecordCache", keep: int, *, sink: int = 128, local: int = 256) -> None:
         """Copy what stays of every sequence and KV head into ``to`` (same
@@ -335,12 +328,9 @@ class RecordCache:
         if self._pages is not None and to._pages is not None and \
                 self.records.data_ptr() == to.records.data_ptr() and not self._pages.isdisjoint(to._pages):
             raise ValueError("the two caches share pages")
-        lib = _hip.load_library()
-        with _hip.on_device(self.device) as stream:
-            size = lib.skv_evict_workspace(self.batch, self.capacity, keep)
-            work = torch.empty(size, dtype=torch.uint8, device=self.device)
-            _hip.check_call("skv_evict", lib.skv_evict(desc, to_desc, keep, sink, local,
-                                                       work.data_ptr(), size, stream))
+        size = _hip.load_library().skv_evict_workspace(self.batch, self.capacity, keep)
+        work = torch.empty(size, dtype=torch.uint8, device=self.device)
+        _hip.call_on(self._index, "skv_evict", desc, to_desc, keep, sink, local, work.data_ptr(), size)
 
     def synchronize(self) -> None:
         """Wait for the device; raise if a write since the last call dropped

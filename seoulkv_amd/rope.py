@@ -19,7 +19,6 @@ position, so far positions cost no accuracy.
 
 from __future__ import annotations
 
-import ctypes
 import math
 from fractions import Fraction
 
@@ -131,30 +130,28 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, table: RotaryTable, *,
     Enqueued on PyTorch's current stream; FP32 arithmetic, rounded once."""
     if not isinstance(table, RotaryTable):
         raise TypeError("table must be a RotaryTable")
-    if x.device.type != "cuda" or x.dtype not in _DTYPES or x.dim() not in (3, 4):
+    shape, dtype = x.shape, _DTYPES.get(x.dtype)
+    if not x.is_cuda or dtype is None or len(shape) not in (3, 4):
         raise ValueError("expected BF16, FP16 or FP32 x [n, heads, dim] or [batch, n, heads, dim] on a GPU")
-    if x.shape[-1] > MAX_HEAD_DIM or x.shape[-1] < table.rotary_dim:
-        raise ValueError(f"head dimension {x.shape[-1]} outside [{table.rotary_dim}, {MAX_HEAD_DIM}]")
-    if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) not in (
-            tuple(x.shape[:-2]), (x.shape[-3],)):
+    if not table.rotary_dim <= shape[-1] <= MAX_HEAD_DIM:
+        raise ValueError(f"head dimension {shape[-1]} outside [{table.rotary_dim}, {MAX_HEAD_DIM}]")
+    if positions.dtype not in (torch.int32, torch.int64) or positions.shape not in (shape[:-2], shape[-3:-2]):
         raise ValueError("expected int32 or int64 positions [n] or [batch, n]")
     if not x.device == positions.device == table.device:
         raise ValueError("x, positions and table must be on one device")
     _no_grad("rotary", x)
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
+        out = x.new_empty(shape)
+    elif out.shape != shape or out.dtype != x.dtype or out.device != x.device:
         raise ValueError("out must have x's shape, type and device")
     if x.numel() == 0:
         return out
     if x.stride(-1) != 1 or out.stride(-1) != 1:
         raise ValueError("the last dimension of x and out must be contiguous")
     positions = positions.contiguous()
-    batch = x.shape[0] if x.dim() == 4 else 1
-    per_batch = x.shape[-3] if positions.dim() == 2 else 0
-    with _hip.on_device(x.device) as stream:
-        _hip.check_call("skv_rotary", _hip.load_library().skv_rotary(
-            ctypes.byref(table._desc), ctypes.byref(_hip.rows_desc(x)), ctypes.byref(_hip.rows_desc(out)),
-            _DTYPES[x.dtype], batch, x.shape[-3], x.shape[-2], x.shape[-1], positions.data_ptr(),
-            per_batch, int(positions.dtype == torch.int64), int(bool(transpose)), stream))
+    batch = shape[0] if len(shape) == 4 else 1
+    per_batch = shape[-3] if positions.dim() == 2 else 0
+    _hip.call_on(x.device.index, "skv_rotary", table._desc, _hip.rows_desc(x), _hip.rows_desc(out),
+                 dtype, batch, x.shape[-3], x.shape[-2], x.shape[-1], positions.data_ptr(), per_batch,
+                 positions.dtype == torch.int64, bool(transpose))
     return out
