@@ -297,7 +297,7 @@ int skv_rotary(const skv_rotary_table *table, const skv_rows *x, const skv_rows 
 
 /* Writes n new tokens of every sequence into slots lengths[b] .. +n-1: V and
  * the turned K as FP8 records (one rounding from FP32), the position and a
- * zero weight where the cache has those arrays.  k, v: BF16 rows [batch][n][4]
+ * zero weight where the cache has those arrays (a position's low 32 bits).  k, v: BF16 rows [batch][n][4]
  * [256].  table NULL: K is stored as given.  q (NULL: none): BF16 rows
  * [batch][n][16][256], turned like K into q_out, BF16 rows that may be q.
  * positions NULL: token i of sequence b has position lengths[b] + i; else
@@ -314,7 +314,7 @@ int skv_cache_write(const skv_record_cache *cache, const skv_rotary_table *table
  * sees every committed slot [0, lengths[b]) and the draft slots lengths[b] + j
  * with j < min(n, counts[b]) and bit j of tree[b][i] set (tree NULL: j <= i, a
  * chain); rows i >= counts[b] see nothing.  q: BF16 rows [batch][n][16][256];
- * score s = q.k / 16, with cap > 0 cap tanh(s / cap); out: BF16
+ * score s = q.k / 16, with cap > 0 (2^-100 .. 2^100) cap tanh(s / cap); out: BF16
  * [batch][n][16][256] = softmax(s) V, lse: FP32 [batch][n][16] = log sum exp
  * s; a row that sees nothing gives 0 and -inf.  workspace: device memory,
  * 16-byte aligned, of skv_tree_workspace(batch, n) bytes. */

@@ -259,7 +259,7 @@ static int tree_operands(Check& c, const skv_record_cache* cache, const skv_rows
   view = view_of(c, cache);
   if (!c.ok()) return c.code;
   c.require(n >= 1 && n <= TREE_MAX_DRAFTS, "%d drafts outside [1, %d]", n, TREE_MAX_DRAFTS);
-  c.require(isfinite(cap) && cap >= 0.f, "cap must be finite and not negative");
+  c.require(cap == 0.f || (cap >= 0x1p-100f && cap <= 0x1p100f), "cap must be 0 or lie in [2^-100, 2^100]");
   if (!c.ok()) return c.code;
   rows = rows_of(c, "q", q, cache->batch, n, QHEADS, SKV_DIM, 2, false);
   if (c.ok())

@@ -227,27 +227,34 @@ __global__ __launch_bounds__(RO_BLOCK) void k_cache_write(WriteArgs a, int64_t i
   auto record = [&](int g) {
     return a.c.records + (a.c.table ? a.c.row_in(page, g, slot) : a.c.row(b, g, slot)) * 512;
   };
-  for (int row = r0; row < min(r1, WR_K); ++row) {
-    const bool is_q = row < WR_Q;
-    if (!is_q && !held) break;
-    const BF16* in = is_q ? source(a.q, row) : source(a.k, row - WR_Q);
+#pragma unroll 4
+  for (int row = r0; row < min(r1, WR_Q); ++row) {
+    const BF16* in = source(a.q, row);
+    BF16* out = const_cast<BF16*>(source(a.q_out, row));
     float f[N], g[N];
     loadn<N>(in + u.lo, f);
     if (u.turned) {
       loadn<N>(in + u.hi, g);
       turn_unit<N, INTER>(f, g, cs);
+      storen<N>(out + u.hi, g);
     }
-    if (is_q) {
-      BF16* out = const_cast<BF16*>(source(a.q_out, row));
-      storen<N>(out + u.lo, f);
-      if (u.turned) storen<N>(out + u.hi, g);
-    } else {
-      uint8_t* out = record(row - WR_Q) + 256;
-      store_fp8<N>(out + u.lo, f);
-      if (u.turned) store_fp8<N>(out + u.hi, g);
-    }
+    storen<N>(out + u.lo, f);
   }
   if (held) {
+#pragma unroll 4
+    for (int row = max(r0, WR_Q); row < min(r1, WR_K); ++row) {
+      const BF16* in = source(a.k, row - WR_Q);
+      uint8_t* out = record(row - WR_Q) + 256;
+      float f[N], g[N];
+      loadn<N>(in + u.lo, f);
+      if (u.turned) {
+        loadn<N>(in + u.hi, g);
+        turn_unit<N, INTER>(f, g, cs);
+        store_fp8<N>(out + u.hi, g);
+      }
+      store_fp8<N>(out + u.lo, f);
+    }
+#pragma unroll 4
     for (int row = max(r0, WR_K); row < r1; ++row) {
       const BF16* in = source(a.v, row - WR_K);
       uint8_t* out = record(row - WR_K);

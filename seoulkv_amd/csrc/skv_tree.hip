@@ -226,26 +226,23 @@ struct ScoreScale {
   // series are exact to 9e-8; where all of a wave's scores are, as is usual,
   // the exponential and the reciprocal are not needed.
   __device__ __forceinline__ void squash(v4f (&s)[2]) const {
-    // tanh(in s) = in s (1 + c[0] s^2 + c[1] s^4 + ..)
+    // tanh x = x (1 + T[0] x^2 + T[1] x^4 + ..)
     constexpr float T[6] = {-1.f / 3.f, 2.f / 15.f, -17.f / 315.f, 62.f / 2835.f, -1382.f / 155925.f,
                             21844.f / 6081075.f};
-    float c[6], power = 1.f;
-#pragma unroll
-    for (int i = 0; i < 6; ++i) c[i] = T[i] * (power *= in * in);
     float most = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(s[e >> 2][e & 3]));
     const bool near = __ballot(!(most * in < 0.5f)) == 0;  // (NaN: passed on either way)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float x = s[e >> 2][e & 3], u = x * x;
-      const float p = x * fmaf(u, fmaf(u, fmaf(u, fmaf(u, fmaf(u, fmaf(u, c[5], c[4]), c[3]), c[2]), c[1]), c[0]), 1.f);
-      s[e >> 2][e & 3] = p;
+      const float x = s[e >> 2][e & 3] * in, u = x * x;
+      float t = x * fmaf(u, fmaf(u, fmaf(u, fmaf(u, fmaf(u, fmaf(u, T[5], T[4]), T[3]), T[2]), T[1]), T[0]), 1.f);
       if (!near) {
-        const float ax = fabsf(x * in);
+        const float ax = fabsf(x);
         const float far = fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(ax * (2.f * DN_LOG2E)) + 1.f), 1.f);
-        s[e >> 2][e & 3] = ax < 0.5f ? p : copysignf(out * far, x);
+        t = ax < 0.5f ? t : copysignf(far, x);
       }
+      s[e >> 2][e & 3] = out * t;
     }
   }
 };
@@ -675,6 +672,7 @@ __global__ __launch_bounds__(512) void k_tree_wide(TreeArgs a) {
       for (int step = 0; step < STEPS; ++step)
         q[rt][step] = __builtin_bit_cast(v8bf, *reinterpret_cast<const uint4*>(src + step_dim(step, kb)));
     }
+    __syncthreads();  // (s_nan is 0 before any wave may set it)
     const int steps = (p1 - p0 + 1) / 2;
     uint4 in[4];
     Tile t;

@@ -54,7 +54,25 @@ class RecordCache:
     tensor; -1: none; capacity = pages x page_tokens).  Sequences may share
     pages that are only read (``write`` and ``evict`` into such a cache
     raise).  ``lengths``: int32 device tensor [batch], kept, or ints.
-    ``positions`` and ``weights``: tensors to keep, or ``None`` to have none."""
+    ``positions`` and ``weights``: tensors to keep, or ``None`` to have none.
+    The kernels read the kept tensors where they lie: change their values in
+    place.  (An int32 ``page_table`` on the device is kept too; the check for
+    shared pages is the constructor's.)"""
+
+    _KEPT = ("records", "lengths", "positions", "weights", "page_table", "status")
+    _desc = None
+
+    def __setattr__(self, name, value):
+        if name in self._KEPT and self._desc is not None and value is not getattr(self, name):
+            raise AttributeError(f"change {name} in place: the kernels read this tensor")
+        object.__setattr__(self, name, value)
+
+    def __enter__(self):
+        self._open()
+        return self
+
+    def __exit__(self, exc_type, exc_value, traceback):
+        self.close()
 
     def __init__(self, records, lengths, *, page_table=None, positions=None, weights=None):
         pool = records if isinstance(records, KVPagePool) else None

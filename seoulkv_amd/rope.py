@@ -109,6 +109,8 @@ class RotaryTable:
         self.layout = layout
         self.turns = _turns(inv).to(dev)
         self.device = self.turns.device
+        # what this constructor enqueued is done before any stream uses it
+        torch.cuda.current_stream(self.device).synchronize()
         self._desc = _hip.RotaryDesc(turns=self.turns.data_ptr(), pairs=rotary_dim // 2,
                                      interleaved=int(layout == "interleaved"), scale=self.scale)
 

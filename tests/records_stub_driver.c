@@ -146,6 +146,8 @@ int main(void) {
   refuse("cap NaN", TREE(&c, &q, 3, NAN, out, lse, work, size), "cap");
   refuse("cap < 0", TREE(&c, &q, 3, -1.f, out, lse, work, size), "cap");
   refuse("cap inf", TREE(&c, &q, 3, INFINITY, out, lse, work, size), "cap");
+  refuse("tiny cap", TREE(&c, &q, 3, 1e-38f, out, lse, work, size), "cap");
+  refuse("huge cap", TREE(&c, &q, 3, 1e38f, out, lse, work, size), "cap");
   refuse("no q", TREE(&c, NULL, 3, 0.f, out, lse, work, size), "NULL q");
   WITH(skv_rows, q, x.data = (char *)x.data + 2, TREE(&c, &x, 3, 0.f, out, lse, work, size), "q by 2", "16-byte");
   WITH(skv_rows, q, x.token_stride = 4097, TREE(&c, &x, 3, 0.f, out, lse, work, size), "odd strides", "16-byte");

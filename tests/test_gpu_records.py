@@ -147,11 +147,21 @@ def test_pages_that_are_none(page_tokens):
     verify(cache, queries(2, 4), random_tree(2, 4))
 
 
-def test_not_a_number_stays_where_it_is_seen():
+@pytest.mark.parametrize("n", [6, 1, 12, 20, 40])
+@pytest.mark.parametrize("length", [45, 3000])
+def test_not_a_number_stays_where_it_is_seen(n, length):
     """NaN records in masked places do not leak; seen ones make NaN of what
     sees them: a dim for one in V, the row for one in K."""
-    n = 6
-    cache = make([45], 64)
+    if n == 1 or length > 45:
+        cache = make([length], length + n + 13)
+        cache.records[0, 0, length + n - 1, 77] = 0x7F
+        cache.records[0, 1, length - 40, 31] = 0xFF  # a committed token's V: every row sees it
+        cache.records[0, 2, length + n:] = 0x7F
+        if n > 1:
+            cache.records[0, 3, length + 1, 256] = 0x7F
+        verify(cache, queries(1, n), random_tree(1, n, seed=21))
+        return
+    cache = make([45], 128)
     tree = random_tree(1, n, seed=21)
     records = cache.records
     records[0, :, 45 + n:] = 0x7F      # behind the drafts
@@ -160,6 +170,30 @@ def test_not_a_number_stays_where_it_is_seen():
     records[0, 2, 45 + n - 1, :] = 0x7F
     records[0, 3, 44, 200] = 0x7F      # V of the last committed token
     verify(cache, queries(1, n), tree)
+
+
+@pytest.mark.parametrize("cap", [1e-6, 0.01, 1.0, 1e6, 1e30])
+def test_caps_of_every_size(cap):
+    """Far under the scores every score is the cap or minus it, far above it
+    none changes."""
+    cache = make([300], 310)
+    q = queries(1, 4)
+    q[0, 0] = 0  # scores of exactly 0
+    if cap >= 1.0:
+        verify(cache, q, cap=cap)
+        if cap >= 1e6:
+            for got, want in zip(cache.tree_decode(q, cap=cap), cache.tree_decode(q)):
+                assert torch.allclose(got.float(), want.float(), rtol=2.0**-7, atol=1e-4)
+    else:  # all but equal weights: the mean of V, to 2 cap
+        out, lse = cache.tree_decode(q, cap=cap)
+        want, want_lse = cache.tree_decode(torch.zeros_like(q))
+        assert torch.isfinite(out).all()
+        # scores move by cap, lse is off by (|lse| + 1) 2^-21 on either side
+        assert float((lse - want_lse).abs().max()) <= cap + 2 * (float(want_lse.abs().max()) + 1) * 2.0**-21
+        # weights move by e^(2 cap) - 1 and are rounded to FP16, the result to BF16
+        size = float(cache.records[..., :256].view(E4M3).float().abs().max())
+        assert float((out.float() - want.float()).abs().max()) <= (
+            size * (2.1 * cap + 2 * 2.0**-11) + 2 * 2.0**-8 * float(want.float().abs().max()))
 
 
 def test_scores_of_every_size():
@@ -566,6 +600,13 @@ def test_refusals():
             call()
     with pytest.raises(TypeError):
         cache.evict(None, 4)
+    for name in ("lengths", "records", "weights"):
+        with pytest.raises(AttributeError, match="in place"):
+            setattr(cache, name, getattr(cache, name).clone())
+    cache.lengths += 0  # in place
+    for cap in (2.0**-120, 2.0**101):
+        with pytest.raises(ValueError, match="cap"):
+            cache.tree_decode(q, cap=cap)
     with pytest.raises(ValueError, match="gradients"):
         cache.tree_decode(q.float().requires_grad_().bfloat16())
     torch.cuda.synchronize()
