@@ -8,7 +8,11 @@
 // Both kernels are bound by memory.  A thread owns 8 pairs (two 16-byte loads
 // in BF16) of one token and keeps their sines and cosines in registers while
 // it walks the heads, so they are formed once per token and not once per
-// head; few tokens are spread over the chip by splitting the heads.
+// head; few tokens are spread over the chip by splitting the heads.  4 heads
+// are in flight at once.  32768 tokens x 20 heads x 256 in BF16: 139 us, 4.8
+// TB/s (torch's copy of as many bytes: 160 us); 32768 tokens into a cache with
+// their queries: 174 us, 4.2 TB/s (188 with one row in flight); a single
+// token of 8 sequences 4.6 us, the launch.
 #include "skv_cache.h"
 #include "skv_device.h"
 

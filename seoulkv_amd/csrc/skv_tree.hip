@@ -9,13 +9,21 @@
 // were off by up to 9e-6 of the sum of magnitudes, BF16 ones by none.)
 // Sums: the lane that holds a score also needs it as column operand of
 // softmax x V, so nothing moves between lanes; V is widened to FP16 (exact)
-// and a probability is rounded once to FP16 (half a step of 2^-10; the running
-// maximum sits at 2^7 .. 2^15, so terms down to 2^-31 of it count).  Sums,
+// and a probability is rounded once to FP16, by at most 2^-11 of itself (the
+// running maximum sits at 2^7 .. 2^15, so terms down to 2^-31 of it count;
+// BF16 would be off by 2^-8, as much as the result's own rounding).  Sums,
 // maxima and row totals are FP32.
 //
 // The sequences' pairs lie in one row, cut into equal shares, one per block:
 // a batch of ragged sequences loads every CU alike.  A share that spans
 // sequences leaves one partial in each; k_tree_merge joins a sequence's.
+//
+// Bounds (131072 keys, contiguous, kernel alone): one to 4 drafts 44.7 us, 6.0
+// TB/s, the record stream; 8 drafts 50, 16 63: the wait for records, since 256
+// registers a wave leave 8 waves a CU and one pair ahead; 32 drafts 115, 64
+// drafts 177, with a cap 210: multiplying and weighing, which two waves a SIMD
+// overlap little (matrix cores busy a quarter of the time at 64 drafts, vector
+// units half).
 #include <type_traits>
 
 #include "skv_cache.h"
@@ -229,21 +237,27 @@ struct ScoreScale {
     // tanh x = x (1 + T[0] x^2 + T[1] x^4 + ..)
     constexpr float T[6] = {-1.f / 3.f, 2.f / 15.f, -17.f / 315.f, 62.f / 2835.f, -1382.f / 155925.f,
                             21844.f / 6081075.f};
-    float most = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(s[e >> 2][e & 3]));
-    const bool near = __ballot(!(most * in < 0.5f)) == 0;  // (NaN: passed on either way)
+    float most = 0.f, x[8], t[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float x = s[e >> 2][e & 3] * in, u = x * x;
-      float t = x * fmaf(u, fmaf(u, fmaf(u, fmaf(u, fmaf(u, fmaf(u, T[5], T[4]), T[3]), T[2]), T[1]), T[0]), 1.f);
-      if (!near) {
-        const float ax = fabsf(x);
-        const float far = fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(ax * (2.f * DN_LOG2E)) + 1.f), 1.f);
-        t = ax < 0.5f ? t : copysignf(far, x);
-      }
-      s[e >> 2][e & 3] = out * t;
+      x[e] = s[e >> 2][e & 3] * in;
+      most = fmaxf(most, fabsf(x[e]));
     }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float u = x[e] * x[e];
+      t[e] = x[e] * fmaf(u, fmaf(u, fmaf(u, fmaf(u, fmaf(u, fmaf(u, T[5], T[4]), T[3]), T[2]), T[1]), T[0]), 1.f);
+    }
+    if (__ballot(!(most < 0.5f))) {  // (fmaxf drops NaN, which the series passes on)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float ax = fabsf(x[e]);
+        const float far = fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(ax * (2.f * DN_LOG2E)) + 1.f), 1.f);
+        t[e] = ax >= 0.5f ? copysignf(far, x[e]) : t[e];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[e >> 2][e & 3] = out * t[e];
   }
 };
 
@@ -781,7 +795,9 @@ __global__ __launch_bounds__(512) void k_tree_wide(TreeArgs a) {
 // (b, g, tile, i / NI)).  SLICES waves each add every SLICES-th share and the
 // slices are added in order: 8 for few sequences, which have up to 64 shares
 // each, with NI 1 where there are few rows too, so that all of a wave's shares
-// are in flight at once; 1 (4 units a block) for many rows with few shares.
+// are in flight at once (one draft, 64 shares: 5.5 us, 8.3 with NI 4); 1 (4
+// units a block) for many rows with few shares (24 sequences x 48 rows: 7.8
+// us, 23.5 when 16 slices had 3.7 shares to add).
 // Where a share met NaN in V among the last keys (it took them as 0), those
 // keys are gone through once more and the dims in which the row sees one
 // become NaN.
@@ -907,8 +923,13 @@ __global__ __launch_bounds__(SLICES == 1 ? 256 : SLICES * 64) void k_tree_merge(
 // ------------------------------------------------------------ key weights
 // A block takes a share of the pairs of KV head g like k_tree's; its waves
 // stride the share, each with all rows of its 32 keys: the queries' image is
-// in LDS, the K halves in registers, and a key's weight is summed over the
-// rows in registers and then over the 16 lanes of a row group.
+// in LDS, the K halves widened once in registers, and a key's weight is summed
+// over the rows in registers and then over the 16 lanes of a row group: no
+// atomics, the same bits every time.  Bound by matrix cores, vector units and
+// LDS about alike for many rows, so 4 waves on a SIMD do more than records
+// loaded ahead (32 rows over 131072 keys: 47 us, 70 with 2 waves and a pair
+// ahead); by the K halves, 256 bytes of every 512, for few (one row 29 us a
+// call, 4.6 TB/s).
 // (the 128 KB image of 64 drafts leaves room for one block, of 16 waves then)
 constexpr int weight_waves(int tiles) { return tiles > 8 ? 16 : 8; }
 
@@ -1025,7 +1046,13 @@ template <bool PAGED>
 void tree_rows(const TreeArgs& a, hipStream_t st) {
   const dim3 grid(TR_BLOCKS, G);
   const int tiles = (a.n * H + 15) / 16;
+  // up to 4 drafts: one tile of rows a wave (49 us a call at 131072 keys; 57
+  // with two, the second empty; 62 with 12 waves, whose 168 registers spill)
   if (tiles <= 1) hipLaunchKernelGGL((k_tree<1, 1, 8, PAGED>), grid, dim3(512), 0, st, a);
+  // two tiles a wave: widened records serve both (16 drafts 70 us, 99 with
+  // one); row waves that hold the same records as far as 32 drafts (118 us,
+  // 139 when they are widened once into LDS), widened once past them (64
+  // drafts 191 us, 219 by 8 row waves each for itself)
   else if (tiles <= 2) hipLaunchKernelGGL((k_tree<2, 1, 8, PAGED>), grid, dim3(512), 0, st, a);
   else if (tiles <= 4) hipLaunchKernelGGL((k_tree<2, 2, 4, PAGED>), grid, dim3(512), 0, st, a);
   else if (tiles <= 8) hipLaunchKernelGGL((k_tree<2, 4, 2, PAGED>), grid, dim3(512), 0, st, a);
