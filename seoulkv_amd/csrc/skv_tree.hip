@@ -21,9 +21,9 @@
 // Bounds (131072 keys, contiguous, kernel alone): one to 4 drafts 44.7 us, 6.0
 // TB/s, the record stream; 8 drafts 50, 16 63: the wait for records, since 256
 // registers a wave leave 8 waves a CU and one pair ahead; 32 drafts 115, 64
-// drafts 177, with a cap 210: multiplying and weighing, which two waves a SIMD
-// overlap little (matrix cores busy a quarter of the time at 64 drafts, vector
-// units half).
+// drafts 169, with a cap 193: multiplying and weighing, which two waves a SIMD
+// overlap little (at 64 capped drafts matrix cores were busy a quarter of the
+// time and vector units 40 %).
 #include <type_traits>
 
 #include "skv_cache.h"
@@ -728,6 +728,10 @@ __global__ __launch_bounds__(512) void k_tree_wide(TreeArgs a) {
         if (lane == 0) s_bad[it & 1][sp * 2 + sx] = t.bad;
       }
     };
+    auto advance = [&](int it) {
+      if (it + 1 < steps) widen(it + 1);
+      if (it + 2 < steps) load(it + 2);
+    };
     load(0);
     widen(0);
     if (steps > 1) load(1);
@@ -735,10 +739,15 @@ __global__ __launch_bounds__(512) void k_tree_wide(TreeArgs a) {
 
     RowSums<RT> sums;
     sums.clear();
-    if (wave >= 4) __builtin_amdgcn_s_setprio(1);  // the two waves of a SIMD drift apart: one multiplies, one weighs
+    if (wave >= 4) __builtin_amdgcn_s_setprio(1);
 #pragma nounroll
     for (int it = 0; it < steps; ++it) {
       const uint4* buf = s_buf + (it & 1) * BUF;
+      // the two waves of a SIMD take turns: one widens the next pairs before it
+      // computes, the other after, and one has priority, so that one weighs
+      // while the other multiplies (64 drafts over 131072 keys 183 us a call;
+      // 189 with the priority alone, 201 with neither)
+      if (wave >= 4) advance(it);
 #pragma nounroll
       for (int pair = 0; pair < 2; ++pair) {
         const int j = p0 + 2 * it + pair;
@@ -779,8 +788,7 @@ __global__ __launch_bounds__(512) void k_tree_wide(TreeArgs a) {
             sums.o[rt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb[rt], sums.o[rt][i], 0, 0, 0);
         }
       }
-      if (it + 1 < steps) widen(it + 1);
-      if (it + 2 < steps) load(it + 2);
+      if (wave < 4) advance(it);
       __syncthreads();
     }
     sums.total();
@@ -1052,7 +1060,7 @@ void tree_rows(const TreeArgs& a, hipStream_t st) {
   // two tiles a wave: widened records serve both (16 drafts 70 us, 99 with
   // one); row waves that hold the same records as far as 32 drafts (118 us,
   // 139 when they are widened once into LDS), widened once past them (64
-  // drafts 191 us, 219 by 8 row waves each for itself)
+  // drafts 183 us, 219 by 8 row waves each for itself)
   else if (tiles <= 2) hipLaunchKernelGGL((k_tree<2, 1, 8, PAGED>), grid, dim3(512), 0, st, a);
   else if (tiles <= 4) hipLaunchKernelGGL((k_tree<2, 2, 4, PAGED>), grid, dim3(512), 0, st, a);
   else if (tiles <= 8) hipLaunchKernelGGL((k_tree<2, 4, 2, PAGED>), grid, dim3(512), 0, st, a);
