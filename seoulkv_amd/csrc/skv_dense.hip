@@ -21,11 +21,21 @@ namespace skv {
 
 namespace {
 
+typedef int v8i __attribute__((ext_vector_type(8)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 
 // A row's running max moves only when a logit exceeds it by more than this
 // (log2 units), so the accumulators are rescaled rarely; p <= 2^DN_TAU.
 constexpr float DN_TAU = 8.f;
+
+__device__ __forceinline__ uint32_t f32_fp8_byte(float x) {
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x, 0.f, 0, false) & 0xffu;
+}
+__device__ __forceinline__ float fp8_byte_f32(uint32_t b) {
+  typedef float v2f __attribute__((ext_vector_type(2)));
+  const v2f f = __builtin_amdgcn_cvt_pk_f32_fp8((int)b, false);
+  return f[0];
+}
 
 // B operand image of the score step, [m][lane][i]: lane l (column c = l % 16
 // = 4h + s, key block kb = l / 16) takes word i of MFMA m, dims
@@ -39,6 +49,10 @@ constexpr float DN_TAU = 8.f;
 constexpr int DN_QWAVES = 8;  // waves that form the image, one word of each MFMA's 8 each
 static_assert(DN_WAVES >= DN_QWAVES, "the query's image is formed by the first 8 waves");
 typedef uint32_t DenseImage[2][WAVE][8];
+
+__device__ __forceinline__ int dn_dim(int m, int i, int kb) {
+  return m * 128 + (i >> 2) * 64 + kb * 16 + (i & 3) * 4;
+}
 
 // The query words a wave needs, loaded ahead of the first tiles: 16 elements
 // of head lane / 16 (for the maxima), and the 4 elements of each of its two
@@ -140,6 +154,10 @@ __device__ __forceinline__ void dn_load_v(DnPair& x, const uint8_t* __restrict__
       x.v[a][r] = load_stream(
           vr + (TAIL ? min(4 * kb + r, a ? last1 : last0) * 512 + 16 * row : vo + 512 * r));
   }
+}
+
+__device__ __forceinline__ v8i as_v8i(uint4 a, uint4 b) {
+  return v8i{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
 }
 
 // The high halves of two words, b's in the low half: two BF16 values.

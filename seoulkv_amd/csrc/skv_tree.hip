@@ -18,12 +18,12 @@
 // a batch of ragged sequences loads every CU alike.  A share that spans
 // sequences leaves one partial in each; k_tree_merge joins a sequence's.
 //
-// Bounds (131072 keys, contiguous, kernel alone): one to 4 drafts 44.7 us, 6.0
-// TB/s, the record stream; 8 drafts 50, 16 63: the wait for records, since 256
-// registers a wave leave 8 waves a CU and one pair ahead; 32 drafts 115, 64
-// drafts 169, with a cap 193: multiplying and weighing, which two waves a SIMD
-// overlap little (at 64 capped drafts matrix cores were busy a quarter of the
-// time and vector units 40 %).
+// Bounds (131072 keys, contiguous, kernel alone): one to 4 drafts 43.7 us, 6.1
+// TB/s, the record stream; 8 drafts 48, 16 61: the wait for records, since 256
+// registers a wave leave 8 waves a CU and one pair ahead; 32 drafts 88, 64
+// drafts 147, with a cap 169: multiplying and weighing, which two waves a SIMD
+// overlap little.  Loads were worth most where no wait stands between their
+// issue and their use: see the loops' notes on branches and spills.
 #include <type_traits>
 
 #include "skv_cache.h"
@@ -56,6 +56,8 @@ struct Sequence {
     drafts = min(k, c.capacity - len);
     keys = len + drafts;
   }
+  // The drafts that are there, as a mask.
+  __device__ __forceinline__ uint64_t there() const { return drafts < 64 ? (1ull << max(drafts, 0)) - 1ull : ~0ull; }
   // The same in scalar registers, for a sequence that the whole wave is at.
   __device__ Sequence uniform() const {
     Sequence s = *this;
@@ -452,15 +454,24 @@ struct RowSums {
   }
 };
 
+// Which of slots len + j .. +3 a row sees (bits 0 .. 3; j > -64) whose mask of
+// the drafts that are there is `bits`.
+__device__ __forceinline__ uint32_t seen4(uint64_t bits, int j) {
+  if (j < 0) bits = (bits << -j) | ((1ull << -j) - 1ull);
+  else bits = j < 64 ? bits >> j : 0ull;
+  return (uint32_t)bits;
+}
+
 // The scores of invisible keys of a pair become -inf: of tiles without a page,
-// and with EDGE of drafts that the row does not see and keys past the end.
+// and with EDGE of drafts that the row does not see (`bits`: those it does) and
+// keys past the end.  j: the lane's first key, from the first draft on.
 template <bool EDGE>
-__device__ __forceinline__ void hide(v4f (&s)[2], const Sequence& seq, uint64_t bits, int at, int kb, bool bad0,
-                                     bool bad1) {
+__device__ __forceinline__ void hide(v4f (&s)[2], uint64_t bits, int j, bool bad0, bool bad1) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const bool seen = !EDGE || sees(seq, bits, at + 16 * (e >> 2) + 4 * kb + (e & 3));
-    if ((e < 4 ? bad0 : bad1) || !seen) s[e >> 2][e & 3] = -INFINITY;
+  for (int x = 0; x < 2; ++x) {
+    const uint32_t seen = (x ? bad1 : bad0) ? 0u : EDGE ? seen4(bits, j + 16 * x) : ~0u;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) s[x][r] = (seen >> r) & 1u ? s[x][r] : -INFINITY;
   }
 }
 
@@ -538,7 +549,7 @@ __global__ __launch_bounds__(RW * KW * 64) void k_tree(TreeArgs a) {
     const int whole = min(p1, first + seq.len / TR_PAIR);  // pairs of committed keys alone come first
     stage_queries<WAVES * 64>(a.q, b, g, TILES, seq.rows, s_buf);
     for (int r = threadIdx.x; r < TILES * 16; r += WAVES * 64)
-      s_bits[r] = r < seq.rows ? row_mask(a.tree, a.n, b, r / H) : 0;
+      s_bits[r] = r < seq.rows ? row_mask(a.tree, a.n, b, r / H) & seq.there() : 0;
     if (threadIdx.x == 0) s_nan = 0;
     Tile t[2];
     uint4 kx[2][4], vx[2][4];
@@ -550,21 +561,21 @@ __global__ __launch_bounds__(RW * KW * 64) void k_tree(TreeArgs a) {
     if (j < whole) {
       tiles(j);
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        load_k<true>(kx[x], t[x], lane);
-        load_v<true>(vx[x], t[x], lane);
-      }
+      for (int x = 0; x < 2; ++x) load_k<true>(kx[x], t[x], lane);
+      __builtin_amdgcn_sched_barrier(0);  // (in the loop's order, which its waits count)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) load_v<true>(vx[x], t[x], lane);
     }
     __syncthreads();
 
     RowSums<RT> sums;
     sums.clear();
     // one pair; EDGE: some of its keys are drafts or past the end (it loads
-    // its records itself)
-    auto step = [&](auto edge) {
-      constexpr bool EDGE = decltype(edge)::value;
+    // its records itself); MORE: the wave's next pair is loaded, by code of its
+    // own, since a wait behind a branch that may not load is one for all loads
+    auto step = [&](auto edge, auto more) {
+      constexpr bool EDGE = decltype(edge)::value, MORE = decltype(more)::value;
       const int at = (j - first) * TR_PAIR;
-      const bool more = !EDGE && j + KW < whole;
       if (EDGE) {
         tiles(j);
 #pragma unroll
@@ -574,7 +585,7 @@ __global__ __launch_bounds__(RW * KW * 64) void k_tree(TreeArgs a) {
         }
       }
       const bool bad0 = t[0].bad, bad1 = t[1].bad;
-      if (more) tiles(j + KW);
+      if (MORE) tiles(j + KW);
       v4f acc[RT][2];
       scores<RT>(kx, s_buf + rw * RT * IMG_TILE, lane, acc);
       // (done before their records' registers are loaded anew)
@@ -582,7 +593,7 @@ __global__ __launch_bounds__(RW * KW * 64) void k_tree(TreeArgs a) {
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
         for (int x = 0; x < 2; ++x) asm volatile("" : "+v"(acc[rt][x]));
-      if (more) {
+      if (MORE) {
 #pragma unroll
         for (int x = 0; x < 2; ++x) load_k<true>(kx[x], t[x], lane);
       }
@@ -591,7 +602,7 @@ __global__ __launch_bounds__(RW * KW * 64) void k_tree(TreeArgs a) {
       for (int rt = 0; rt < RT; ++rt) {
         if (cap) zs.squash(acc[rt]);
         if (EDGE || bad0 || bad1)
-          hide<EDGE>(acc[rt], seq, EDGE ? s_bits[(rw * RT + rt) * 16 + col] : 0, at, kb, bad0, bad1);
+          hide<EDGE>(acc[rt], EDGE ? s_bits[(rw * RT + rt) * 16 + col] : 0, at + 4 * kb - seq.len, bad0, bad1);
         pb[rt] = sums.weigh(rt, acc[rt], zs.unit);
       }
       if (bad0 || bad1) {
@@ -621,16 +632,17 @@ __global__ __launch_bounds__(RW * KW * 64) void k_tree(TreeArgs a) {
                 __builtin_amdgcn_mfma_f32_16x16x32_f16(va[i], pb[rt], sums.o[rt][4 * w + i], 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);  // one word's operands live at a time
       }
-      if (more) {
+      if (MORE) {
 #pragma unroll
         for (int x = 0; x < 2; ++x) load_v<true>(vx[x], t[x], lane);
       }
       j += KW;
     };
 #pragma nounroll
-    while (j < whole) step(std::false_type{});
+    while (j + KW < whole) step(std::false_type{}, std::true_type{});
+    if (j < whole) step(std::false_type{}, std::false_type{});
 #pragma nounroll
-    while (j < p1) step(std::true_type{});
+    while (j < p1) step(std::true_type{}, std::false_type{});
     sums.total();
     sums.template join<RW>(min(KW, p1 - p0), rw, kw, seq.rows, lane, s_buf, s_ml);  // (waves without a pair hold nothing)
     const Partials part = partials();
@@ -641,19 +653,19 @@ __global__ __launch_bounds__(RW * KW * 64) void k_tree(TreeArgs a) {
   });
 }
 
-// More than 32 drafts: 8 row waves of 32 rows would each widen the same
+// More than 16 drafts: 8 row waves of 16 RT rows would each widen the same
 // records.  Here they load and widen two pairs together into LDS, twice
 // buffered, and every wave reads its operands there; the queries stay in
 // registers.
-template <bool PAGED>
+template <int RT, bool PAGED>
 __global__ __launch_bounds__(512) void k_tree_wide(TreeArgs a) {
-  constexpr int RT = 2, TILES = 16;
+  constexpr int TILES = RT * 8;
   constexpr int KBUF = 2 * 2 * IMG_TILE;   // uint4: [pair][tile][step][lane]
   constexpr int VBUF = 2 * 16 * WAVE;      // uint4: [pair][dim of 16][lane], tile x in half x
   constexpr int BUF = KBUF + VBUF;         // 64 KB
   __shared__ uint4 s_buf[2 * BUF];
   __shared__ uint64_t s_bits[TILES * 16];
-  __shared__ int s_bad[2][4];
+  __shared__ uint32_t s_bad[2];  // of the four tiles in a buffer, a byte each
   __shared__ int s_start[CACHE_MAX_BATCH + 1];
   __shared__ int s_nan;
   const int g = blockIdx.y, k = blockIdx.x;
@@ -673,7 +685,7 @@ __global__ __launch_bounds__(512) void k_tree_wide(TreeArgs a) {
   each_piece(a, s_start, [&](int b, int first, int p0, int p1) {
     const Sequence seq = Sequence(a.c, a.counts, a.n, b).uniform();
     for (int r = threadIdx.x; r < TILES * 16; r += 512)
-      s_bits[r] = r < seq.rows ? row_mask(a.tree, a.n, b, r / H) : 0;
+      s_bits[r] = r < seq.rows ? row_mask(a.tree, a.n, b, r / H) & seq.there() : 0;
     if (threadIdx.x == 0) s_nan = 0;
     v8bf q[RT][STEPS];
 #pragma unroll
@@ -686,19 +698,37 @@ __global__ __launch_bounds__(512) void k_tree_wide(TreeArgs a) {
       for (int step = 0; step < STEPS; ++step)
         q[rt][step] = __builtin_bit_cast(v8bf, *reinterpret_cast<const uint4*>(src + step_dim(step, kb)));
     }
+    // waited for here: a wait in the loop would be one for the records too
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int step = 0; step < STEPS; ++step) asm volatile("" : "+v"(q[rt][step]));
     __syncthreads();  // (s_nan is 0 before any wave may set it)
     const int steps = (p1 - p0 + 1) / 2;
     uint4 in[4];
     Tile t;
+    // (formed anew where it is used: what is made of it does not stay in
+    // registers; a spill of loaded records would wait for them)
+    auto anew = [](int x) {
+      asm volatile("" : "+v"(x));
+      return x;
+    };
+    // K and V through one code path: registers that two branches load are
+    // copied where the branches meet, which waits for the loads
     auto load = [&](int it) {  // (past the last pair: its last tile again, not used)
       const int pair = min(p0 + 2 * it + sp, p1 - 1);
       t = tile_at<PAGED>(a.c, b, g, (pair - first) * TR_PAIR + 16 * sx, seq.keys);
-      if (sv) load_v<false>(in, t, lane);
-      else load_k<false>(in, t, lane);
+      const int ln = anew(lane), col = ln & 15, kb = ln >> 4;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint32_t at = min(sv ? 4 * kb + r : col, t.last) * 512 + (sv ? 16 * col : 256 + 64 * r + 16 * kb);
+        in[r] = *reinterpret_cast<const uint4*>(t.at + at);
+      }
     };
     auto widen = [&](int it) {
       uint4* buf = s_buf + (it & 1) * BUF;
       const int pair = min(p0 + 2 * it + sp, p1 - 1);
+      const int lane = anew(threadIdx.x) & 63;
       if (sv) {
         if (PAGED && t.bad) {
 #pragma unroll
@@ -725,7 +755,7 @@ __global__ __launch_bounds__(512) void k_tree_wide(TreeArgs a) {
           const uint4 w = in[step >> 1];
           out[step * WAVE] = __builtin_bit_cast(uint4, (step & 1) ? k_operand(w.z, w.w) : k_operand(w.x, w.y));
         }
-        if (lane == 0) s_bad[it & 1][sp * 2 + sx] = t.bad;
+        if (PAGED && lane == 0) reinterpret_cast<uint8_t*>(&s_bad[it & 1])[sp * 2 + sx] = t.bad;
       }
     };
     auto advance = [&](int it) {
@@ -743,16 +773,20 @@ __global__ __launch_bounds__(512) void k_tree_wide(TreeArgs a) {
 #pragma nounroll
     for (int it = 0; it < steps; ++it) {
       const uint4* buf = s_buf + (it & 1) * BUF;
+      uint32_t bad = 0;  // a byte for each of the buffer's tiles
+      if constexpr (PAGED) bad = __builtin_amdgcn_readfirstlane(s_bad[it & 1]);
       // the two waves of a SIMD take turns: one widens the next pairs before it
       // computes, the other after, and one has priority, so that one weighs
-      // while the other multiplies (64 drafts over 131072 keys 183 us a call;
-      // 189 with the priority alone, 201 with neither)
+      // while the other multiplies (64 drafts over 131072 keys: 201 us a call
+      // without, 189 with the priority alone, 183 with both, before the waits
+      // for records were taken out)
       if (wave >= 4) advance(it);
 #pragma nounroll
       for (int pair = 0; pair < 2; ++pair) {
         const int j = p0 + 2 * it + pair;
         if (j >= p1) break;
         const int at = (j - first) * TR_PAIR;
+        const int ln = anew(lane);
         v4f acc[RT][2];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) acc[rt][0] = acc[rt][1] = v4f{0.f, 0.f, 0.f, 0.f};
@@ -760,26 +794,24 @@ __global__ __launch_bounds__(512) void k_tree_wide(TreeArgs a) {
         for (int step = 0; step < STEPS; ++step)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            const v8bf kk = __builtin_bit_cast(v8bf, buf[((pair * 2 + x) * STEPS + step) * WAVE + lane]);
+            const v8bf kk = __builtin_bit_cast(v8bf, buf[((pair * 2 + x) * STEPS + step) * WAVE + ln]);
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
               acc[rt][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kk, q[rt][step], acc[rt][x], 0, 0, 0);
           }
         const bool edge = at + TR_PAIR > seq.len;
-        bool bad0 = false, bad1 = false;
-        if constexpr (PAGED) {
-          bad0 = __builtin_amdgcn_readfirstlane(s_bad[it & 1][pair * 2]) != 0;
-          bad1 = __builtin_amdgcn_readfirstlane(s_bad[it & 1][pair * 2 + 1]) != 0;
-        }
+        const bool bad0 = (bad >> (16 * pair)) & 0xffu, bad1 = (bad >> (16 * pair + 8)) & 0xffu;
         v8h pb[RT];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
           if (cap) zs.squash(acc[rt]);
-          if (edge) hide<true>(acc[rt], seq, s_bits[(wave * RT + rt) * 16 + col], at, kb, bad0, bad1);
-          else if (bad0 || bad1) hide<false>(acc[rt], seq, 0, at, kb, bad0, bad1);
+          if (edge)
+            hide<true>(acc[rt], s_bits[(wave * RT + rt) * 16 + (ln & 15)], at + 4 * (ln >> 4) - seq.len, bad0, bad1);
+          else if (bad0 || bad1)
+            hide<false>(acc[rt], 0, 0, bad0, bad1);
           pb[rt] = sums.weigh(rt, acc[rt], zs.unit);
         }
-        const uint4* vb = buf + KBUF + pair * 16 * WAVE + lane;
+        const uint4* vb = buf + KBUF + pair * 16 * WAVE + ln;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const v8h va = __builtin_bit_cast(v8h, vb[i * WAVE]);
@@ -1057,14 +1089,15 @@ void tree_rows(const TreeArgs& a, hipStream_t st) {
   // up to 4 drafts: one tile of rows a wave (49 us a call at 131072 keys; 57
   // with two, the second empty; 62 with 12 waves, whose 168 registers spill)
   if (tiles <= 1) hipLaunchKernelGGL((k_tree<1, 1, 8, PAGED>), grid, dim3(512), 0, st, a);
-  // two tiles a wave: widened records serve both (16 drafts 70 us, 99 with
-  // one); row waves that hold the same records as far as 32 drafts (118 us,
-  // 139 when they are widened once into LDS), widened once past them (64
-  // drafts 183 us, 219 by 8 row waves each for itself)
+  // two tiles a wave: widened records serve both (16 drafts 69 us, 99 with
+  // one); row waves that hold the same records as far as 16 drafts (64 ragged
+  // paged sequences of 2000 keys 75 us, 84 when they are widened once into
+  // LDS), widened once past them (32 drafts 95 us, 122 by 4 row waves each for
+  // itself; 64 drafts 160 us, 219 by 8)
   else if (tiles <= 2) hipLaunchKernelGGL((k_tree<2, 1, 8, PAGED>), grid, dim3(512), 0, st, a);
   else if (tiles <= 4) hipLaunchKernelGGL((k_tree<2, 2, 4, PAGED>), grid, dim3(512), 0, st, a);
-  else if (tiles <= 8) hipLaunchKernelGGL((k_tree<2, 4, 2, PAGED>), grid, dim3(512), 0, st, a);
-  else hipLaunchKernelGGL(k_tree_wide<PAGED>, grid, dim3(512), 0, st, a);
+  else if (tiles <= 8) hipLaunchKernelGGL((k_tree_wide<1, PAGED>), grid, dim3(512), 0, st, a);
+  else hipLaunchKernelGGL((k_tree_wide<2, PAGED>), grid, dim3(512), 0, st, a);
 }
 
 template <bool PAGED>
