@@ -18,12 +18,13 @@
 // a batch of ragged sequences loads every CU alike.  A share that spans
 // sequences leaves one partial in each; k_tree_merge joins a sequence's.
 //
-// Bounds (131072 keys, contiguous, kernel alone): one to 4 drafts 43.7 us, 6.1
-// TB/s, the record stream; 8 drafts 48, 16 61: the wait for records, since 256
-// registers a wave leave 8 waves a CU and one pair ahead; 32 drafts 88, 64
-// drafts 147, with a cap 169: multiplying and weighing, which two waves a SIMD
-// overlap little.  Loads were worth most where no wait stands between their
-// issue and their use: see the loops' notes on branches and spills.
+// Bounds (131072 keys, contiguous, a whole call): one to 4 drafts 49 us, of
+// which the kernel 44, 6.0 TB/s, the record stream; 8 drafts 54, 16 68: the wait
+// for records, since 256 registers a wave leave 8 waves a CU and one pair ahead;
+// 32 drafts 95, 64 drafts 155, with a cap 178: multiplying and weighing, which
+// two waves a SIMD overlap little (loads two or three steps ahead changed
+// nothing there).  Loads pay where no wait stands between their issue and their
+// use: see the loops' notes on branches and spills.
 #include <type_traits>
 
 #include "skv_cache.h"
@@ -705,123 +706,127 @@ __global__ __launch_bounds__(512) void k_tree_wide(TreeArgs a) {
       for (int step = 0; step < STEPS; ++step) asm volatile("" : "+v"(q[rt][step]));
     __syncthreads();  // (s_nan is 0 before any wave may set it)
     const int steps = (p1 - p0 + 1) / 2;
-    uint4 in[4];
-    Tile t;
     // (formed anew where it is used: what is made of it does not stay in
     // registers; a spill of loaded records would wait for them)
     auto anew = [](int x) {
       asm volatile("" : "+v"(x));
       return x;
     };
-    // K and V through one code path: registers that two branches load are
-    // copied where the branches meet, which waits for the loads
-    auto load = [&](int it) {  // (past the last pair: its last tile again, not used)
-      const int pair = min(p0 + 2 * it + sp, p1 - 1);
-      t = tile_at<PAGED>(a.c, b, g, (pair - first) * TR_PAIR + 16 * sx, seq.keys);
-      const int ln = anew(lane), col = ln & 15, kb = ln >> 4;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const uint32_t at = min(sv ? 4 * kb + r : col, t.last) * 512 + (sv ? 16 * col : 256 + 64 * r + 16 * kb);
-        in[r] = *reinterpret_cast<const uint4*>(t.at + at);
-      }
-    };
-    auto widen = [&](int it) {
-      uint4* buf = s_buf + (it & 1) * BUF;
-      const int pair = min(p0 + 2 * it + sp, p1 - 1);
-      const int lane = anew(threadIdx.x) & 63;
-      if (sv) {
-        if (PAGED && t.bad) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) in[r] = make_uint4(0, 0, 0, 0);
-        }
-        if ((pair - first + 1) * TR_PAIR > seq.len) {
-          uint32_t any = 0;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) any |= drop_nan(in[r]);
-          if (__ballot(any != 0) && lane == 0) s_nan = 1;
-        }
-        uint2* out = reinterpret_cast<uint2*>(buf + KBUF + sp * 16 * WAVE + lane) + sx;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          uint2 half[4];
-          v_halves(in, w, half);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) out[(4 * w + i) * WAVE * 2] = half[i];
-        }
-      } else {
-        uint4* out = buf + (sp * 2 + sx) * IMG_TILE + lane;
-#pragma unroll
-        for (int step = 0; step < STEPS; ++step) {
-          const uint4 w = in[step >> 1];
-          out[step * WAVE] = __builtin_bit_cast(uint4, (step & 1) ? k_operand(w.z, w.w) : k_operand(w.x, w.y));
-        }
-        if (PAGED && lane == 0) reinterpret_cast<uint8_t*>(&s_bad[it & 1])[sp * 2 + sx] = t.bad;
-      }
-    };
-    auto advance = [&](int it) {
-      if (it + 1 < steps) widen(it + 1);
-      if (it + 2 < steps) load(it + 2);
-    };
-    load(0);
-    widen(0);
-    if (steps > 1) load(1);
-    __syncthreads();
-
     RowSums<RT> sums;
     sums.clear();
-    if (wave >= 4) __builtin_amdgcn_s_setprio(1);
+    // What a wave does, in two forms, of waves that load and widen K and of
+    // those that do V: registers that two branches load are copied where the
+    // branches meet, which waits for the loads.  Both take the same barriers.
+    auto walk = [&](auto values) {
+      constexpr bool V = decltype(values)::value;
+      uint4 in[4];
+      Tile t;
+      auto load = [&](int it) {  // (past the last pair: its last tile again, not used)
+        const int pair = min(p0 + 2 * it + sp, p1 - 1);
+        t = tile_at<PAGED>(a.c, b, g, (pair - first) * TR_PAIR + 16 * sx, seq.keys);
+        if (V) load_v<false>(in, t, anew(lane));
+        else load_k<false>(in, t, anew(lane));
+      };
+      auto widen = [&](int it) {
+        uint4* buf = s_buf + (it & 1) * BUF;
+        const int pair = min(p0 + 2 * it + sp, p1 - 1);
+        const int lane = anew(threadIdx.x) & 63;
+        if (V) {
+          if (PAGED && t.bad) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) in[r] = make_uint4(0, 0, 0, 0);
+          }
+          if ((pair - first + 1) * TR_PAIR > seq.len) {
+            uint32_t any = 0;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) any |= drop_nan(in[r]);
+            if (__ballot(any != 0) && lane == 0) s_nan = 1;
+          }
+          uint2* out = reinterpret_cast<uint2*>(buf + KBUF + sp * 16 * WAVE + lane) + sx;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            uint2 half[4];
+            v_halves(in, w, half);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) out[(4 * w + i) * WAVE * 2] = half[i];
+          }
+        } else {
+          uint4* out = buf + (sp * 2 + sx) * IMG_TILE + lane;
+#pragma unroll
+          for (int step = 0; step < STEPS; ++step) {
+            const uint4 w = in[step >> 1];
+            out[step * WAVE] = __builtin_bit_cast(uint4, (step & 1) ? k_operand(w.z, w.w) : k_operand(w.x, w.y));
+          }
+          if (PAGED && lane == 0) reinterpret_cast<uint8_t*>(&s_bad[it & 1])[sp * 2 + sx] = t.bad;
+        }
+      };
+      auto advance = [&](int it) {
+        if (it + 1 < steps) widen(it + 1);
+        if (it + 2 < steps) load(it + 2);
+      };
+      load(0);
+      widen(0);
+      if (steps > 1) load(1);
+      __syncthreads();
 #pragma nounroll
-    for (int it = 0; it < steps; ++it) {
-      const uint4* buf = s_buf + (it & 1) * BUF;
-      uint32_t bad = 0;  // a byte for each of the buffer's tiles
-      if constexpr (PAGED) bad = __builtin_amdgcn_readfirstlane(s_bad[it & 1]);
-      // the two waves of a SIMD take turns: one widens the next pairs before it
-      // computes, the other after, and one has priority, so that one weighs
-      // while the other multiplies (64 drafts over 131072 keys: 201 us a call
-      // without, 189 with the priority alone, 183 with both, before the waits
-      // for records were taken out)
-      if (wave >= 4) advance(it);
+      for (int it = 0; it < steps; ++it) {
+        const uint4* buf = s_buf + (it & 1) * BUF;
+        uint32_t bad = 0;  // a byte for each of the buffer's tiles
+        if constexpr (PAGED) bad = __builtin_amdgcn_readfirstlane(s_bad[it & 1]);
+        // the two waves of a SIMD take turns: one widens the next pairs before
+        // it computes, the other after, and one has priority, so that one
+        // weighs while the other multiplies (64 drafts over 131072 keys: 201 us
+        // a call without, 189 with the priority alone, 183 with both, before
+        // the waits for records were taken out)
+        if (V) advance(it);
 #pragma nounroll
-      for (int pair = 0; pair < 2; ++pair) {
-        const int j = p0 + 2 * it + pair;
-        if (j >= p1) break;
-        const int at = (j - first) * TR_PAIR;
-        const int ln = anew(lane);
-        v4f acc[RT][2];
+        for (int pair = 0; pair < 2; ++pair) {
+          const int j = p0 + 2 * it + pair;
+          if (j >= p1) break;
+          const int at = (j - first) * TR_PAIR;
+          const int ln = anew(lane);
+          v4f acc[RT][2];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) acc[rt][0] = acc[rt][1] = v4f{0.f, 0.f, 0.f, 0.f};
+          for (int rt = 0; rt < RT; ++rt) acc[rt][0] = acc[rt][1] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int step = 0; step < STEPS; ++step)
+          for (int step = 0; step < STEPS; ++step)
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const v8bf kk = __builtin_bit_cast(v8bf, buf[((pair * 2 + x) * STEPS + step) * WAVE + ln]);
+            for (int x = 0; x < 2; ++x) {
+              const v8bf kk = __builtin_bit_cast(v8bf, buf[((pair * 2 + x) * STEPS + step) * WAVE + ln]);
+#pragma unroll
+              for (int rt = 0; rt < RT; ++rt)
+                acc[rt][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kk, q[rt][step], acc[rt][x], 0, 0, 0);
+            }
+          const bool edge = at + TR_PAIR > seq.len;
+          const bool bad0 = (bad >> (16 * pair)) & 0xffu, bad1 = (bad >> (16 * pair + 8)) & 0xffu;
+          v8h pb[RT];
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) {
+            if (cap) zs.squash(acc[rt]);
+            if (edge)
+              hide<true>(acc[rt], s_bits[(wave * RT + rt) * 16 + (ln & 15)], at + 4 * (ln >> 4) - seq.len, bad0, bad1);
+            else if (bad0 || bad1)
+              hide<false>(acc[rt], 0, 0, bad0, bad1);
+            pb[rt] = sums.weigh(rt, acc[rt], zs.unit);
+          }
+          const uint4* vb = buf + KBUF + pair * 16 * WAVE + ln;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const v8h va = __builtin_bit_cast(v8h, vb[i * WAVE]);
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
-              acc[rt][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kk, q[rt][step], acc[rt][x], 0, 0, 0);
+              sums.o[rt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb[rt], sums.o[rt][i], 0, 0, 0);
           }
-        const bool edge = at + TR_PAIR > seq.len;
-        const bool bad0 = (bad >> (16 * pair)) & 0xffu, bad1 = (bad >> (16 * pair + 8)) & 0xffu;
-        v8h pb[RT];
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          if (cap) zs.squash(acc[rt]);
-          if (edge)
-            hide<true>(acc[rt], s_bits[(wave * RT + rt) * 16 + (ln & 15)], at + 4 * (ln >> 4) - seq.len, bad0, bad1);
-          else if (bad0 || bad1)
-            hide<false>(acc[rt], 0, 0, bad0, bad1);
-          pb[rt] = sums.weigh(rt, acc[rt], zs.unit);
         }
-        const uint4* vb = buf + KBUF + pair * 16 * WAVE + ln;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const v8h va = __builtin_bit_cast(v8h, vb[i * WAVE]);
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt)
-            sums.o[rt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb[rt], sums.o[rt][i], 0, 0, 0);
-        }
+        if (!V) advance(it);
+        __syncthreads();
       }
-      if (wave < 4) advance(it);
-      __syncthreads();
+    };
+    if (sv) {
+      __builtin_amdgcn_s_setprio(1);
+      walk(std::true_type{});
+    } else {
+      walk(std::false_type{});
     }
     sums.total();
     const Partials part = partials();
@@ -1093,7 +1098,7 @@ void tree_rows(const TreeArgs& a, hipStream_t st) {
   // one); row waves that hold the same records as far as 16 drafts (64 ragged
   // paged sequences of 2000 keys 75 us, 84 when they are widened once into
   // LDS), widened once past them (32 drafts 95 us, 122 by 4 row waves each for
-  // itself; 64 drafts 160 us, 219 by 8)
+  // itself; 64 drafts 155 us, 219 by 8)
   else if (tiles <= 2) hipLaunchKernelGGL((k_tree<2, 1, 8, PAGED>), grid, dim3(512), 0, st, a);
   else if (tiles <= 4) hipLaunchKernelGGL((k_tree<2, 2, 4, PAGED>), grid, dim3(512), 0, st, a);
   else if (tiles <= 8) hipLaunchKernelGGL((k_tree_wide<1, PAGED>), grid, dim3(512), 0, st, a);
