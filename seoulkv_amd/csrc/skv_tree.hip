@@ -1095,8 +1095,8 @@ void tree_rows(const TreeArgs& a, hipStream_t st) {
   // with two, the second empty; 62 with 12 waves, whose 168 registers spill)
   if (tiles <= 1) hipLaunchKernelGGL((k_tree<1, 1, 8, PAGED>), grid, dim3(512), 0, st, a);
   // two tiles a wave: widened records serve both (16 drafts 69 us, 99 with
-  // one); row waves that hold the same records as far as 16 drafts (64 ragged
-  // paged sequences of 2000 keys 75 us, 84 when they are widened once into
+  // one); row waves that hold the same records as far as 16 drafts (12 in 64
+  // paged sequences of 2000 keys 76 us, 80 when they are widened once into
   // LDS), widened once past them (32 drafts 95 us, 122 by 4 row waves each for
   // itself; 64 drafts 155 us, 219 by 8)
   else if (tiles <= 2) hipLaunchKernelGGL((k_tree<2, 1, 8, PAGED>), grid, dim3(512), 0, st, a);
