@@ -19,7 +19,7 @@
 // sequences leaves one partial in each; k_tree_merge joins a sequence's.
 //
 // Bounds (131072 keys, contiguous, a whole call): one to 4 drafts 49 us, of
-// which the kernel 44, 6.0 TB/s, the record stream; 8 drafts 54, 16 68: the wait
+// which the kernel 44, 6.0 TB/s, the record stream; 8 drafts 54, 16 66: the wait
 // for records, since 256 registers a wave leave 8 waves a CU and one pair ahead;
 // 32 drafts 95, 64 drafts 155, with a cap 178: multiplying and weighing, which
 // two waves a SIMD overlap little (loads two or three steps ahead changed
@@ -149,12 +149,16 @@ __device__ __forceinline__ void load_k(uint4 (&k)[4], const Tile& x, int lane) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) k[j] = *reinterpret_cast<const uint4*>(x.at + 256 + 64 * j + at);
 }
-template <bool WHOLE>
+// ONCE: no other wave reads the tile.  Where two row waves do, streaming loads
+// brought a fifth of the records from memory twice (12 drafts of 24 ragged
+// sequences: 557 MB and 124 us, 455 MB and 118 us with plain ones).
+template <bool WHOLE, bool ONCE>
 __device__ __forceinline__ void load_v(uint4 (&v)[4], const Tile& x, int lane) {
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const int row = 4 * (lane >> 4) + r;
-    v[r] = load_stream(x.at + (uint32_t)((WHOLE ? row : min(row, x.last)) * 512 + 16 * (lane & 15)));
+    const uint8_t* at = x.at + (uint32_t)((WHOLE ? row : min(row, x.last)) * 512 + 16 * (lane & 15));
+    v[r] = ONCE ? load_stream(at) : *reinterpret_cast<const uint4*>(at);
   }
 }
 
@@ -565,7 +569,7 @@ __global__ __launch_bounds__(RW * KW * 64) void k_tree(TreeArgs a) {
       for (int x = 0; x < 2; ++x) load_k<true>(kx[x], t[x], lane);
       __builtin_amdgcn_sched_barrier(0);  // (in the loop's order, which its waits count)
 #pragma unroll
-      for (int x = 0; x < 2; ++x) load_v<true>(vx[x], t[x], lane);
+      for (int x = 0; x < 2; ++x) load_v<true, RW == 1>(vx[x], t[x], lane);
     }
     __syncthreads();
 
@@ -582,7 +586,7 @@ __global__ __launch_bounds__(RW * KW * 64) void k_tree(TreeArgs a) {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           load_k<false>(kx[x], t[x], lane);
-          load_v<false>(vx[x], t[x], lane);
+          load_v<false, RW == 1>(vx[x], t[x], lane);
         }
       }
       const bool bad0 = t[0].bad, bad1 = t[1].bad;
@@ -635,7 +639,7 @@ __global__ __launch_bounds__(RW * KW * 64) void k_tree(TreeArgs a) {
       }
       if (MORE) {
 #pragma unroll
-        for (int x = 0; x < 2; ++x) load_v<true>(vx[x], t[x], lane);
+        for (int x = 0; x < 2; ++x) load_v<true, RW == 1>(vx[x], t[x], lane);
       }
       j += KW;
     };
@@ -724,7 +728,7 @@ __global__ __launch_bounds__(512) void k_tree_wide(TreeArgs a) {
       auto load = [&](int it) {  // (past the last pair: its last tile again, not used)
         const int pair = min(p0 + 2 * it + sp, p1 - 1);
         t = tile_at<PAGED>(a.c, b, g, (pair - first) * TR_PAIR + 16 * sx, seq.keys);
-        if (V) load_v<false>(in, t, anew(lane));
+        if (V) load_v<false, true>(in, t, anew(lane));
         else load_k<false>(in, t, anew(lane));
       };
       auto widen = [&](int it) {
@@ -1094,9 +1098,9 @@ void tree_rows(const TreeArgs& a, hipStream_t st) {
   // up to 4 drafts: one tile of rows a wave (49 us a call at 131072 keys; 57
   // with two, the second empty; 62 with 12 waves, whose 168 registers spill)
   if (tiles <= 1) hipLaunchKernelGGL((k_tree<1, 1, 8, PAGED>), grid, dim3(512), 0, st, a);
-  // two tiles a wave: widened records serve both (16 drafts 69 us, 99 with
+  // two tiles a wave: widened records serve both (16 drafts 66 us, 99 with
   // one); row waves that hold the same records as far as 16 drafts (12 in 64
-  // paged sequences of 2000 keys 76 us, 80 when they are widened once into
+  // paged sequences of 2000 keys 72 us, 80 when they are widened once into
   // LDS), widened once past them (32 drafts 95 us, 122 by 4 row waves each for
   // itself; 64 drafts 155 us, 219 by 8)
   else if (tiles <= 2) hipLaunchKernelGGL((k_tree<2, 1, 8, PAGED>), grid, dim3(512), 0, st, a);
