@@ -334,11 +334,13 @@ int skv_key_weights(const skv_record_cache *cache, const skv_rows *q, int n, con
 
 /* Copies what stays of every sequence and KV head into slots 0 .. m-1 of
  * another cache `to` (same batch, capacity >= keep, other memory), in slot
- * order: m = min(lengths[b], keep) slots, the first `sink` and the last
- * `local` committed ones and of the rest those with the largest weights (ties:
- * the lowest slot; NaN counts as the least).  Positions and weights go along
- * (where both caches have them; the source must have weights); to->lengths[b] = m.  keep >= sink + local, keep >= 1.  The
- * source is not changed.  workspace: device memory, 16-byte aligned, of
+ * order.  Slots whose page is none hold no key and are passed over: of the
+ * other committed slots of sequence b m = min(their number, keep) stay, the
+ * first `sink`, the last `local` and of the rest those with the largest weights
+ * (ties: the lowest slot; NaN counts as the least).  Positions and weights go
+ * along (where both caches have them; the source must have weights);
+ * to->lengths[b] = m.  keep >= sink + local, keep >= 1.  The source is not
+ * changed.  workspace: device memory, 16-byte aligned, of
  * skv_evict_workspace(batch, capacity, keep) bytes. */
 int skv_evict(const skv_record_cache *cache, const skv_record_cache *to, int keep, int sink,
               int local, void *workspace, int64_t workspace_bytes, void *stream);

@@ -106,8 +106,12 @@ struct EvictArgs {
   int* to_lengths;
   int keep, sink, local;
   void* workspace;
+  // in the workspace, set by launch_evict: per list the slots that have a page,
+  // and those before each page
+  int *held, *before;
+  int before_stride;
 };
 size_t evict_workspace(int batch, int capacity, int keep);
-void launch_evict(const EvictArgs& a, hipStream_t st);
+void launch_evict(EvictArgs a, hipStream_t st);
 
 }  // namespace skv

@@ -328,8 +328,9 @@ class RecordCache:
         batch, other memory), in slot order: at most ``keep`` slots, the first
         ``sink``, the last ``local`` committed ones and of the rest the
         heaviest by ``weights`` (ties: the lowest slot; NaN counts least).
-        Records, positions and weights go along and ``to.lengths`` is set;
-        this cache does not change.  Heads keep different tokens:
+        Slots whose page is none hold no key: they are passed over and count
+        nowhere.  Records, positions and weights go along and ``to.lengths``
+        is set; this cache does not change.  Heads keep different tokens:
         ``to.positions`` says which (needs positions in both caches)."""
         if not isinstance(to, RecordCache):
             raise TypeError("expected a RecordCache to evict into")
