@@ -339,7 +339,8 @@ int skv_key_weights(const skv_record_cache *cache, const skv_rows *q, int n, con
  * first `sink`, the last `local` and of the rest those with the largest weights
  * (ties: the lowest slot; NaN counts as the least).  Positions and weights go
  * along (where both caches have them; the source must have weights);
- * to->lengths[b] = m.  keep >= sink + local, keep >= 1.  The source is not
+ * to->lengths[b] = m.  What falls on a slot of `to` without a page is dropped,
+ * with a bit in to->status.  keep >= sink + local, keep >= 1.  The source is not
  * changed.  workspace: device memory, 16-byte aligned, of
  * skv_evict_workspace(batch, capacity, keep) bytes. */
 int skv_evict(const skv_record_cache *cache, const skv_record_cache *to, int keep, int sink,

@@ -104,6 +104,7 @@ struct EvictArgs {
   int* to_positions;  // NULL: not copied
   float* to_weights;
   int* to_lengths;
+  int* to_status;  // NULL: not noted
   int keep, sink, local;
   void* workspace;
   // in the workspace, set by launch_evict: per list the slots that have a page,

@@ -357,6 +357,7 @@ int skv_evict(const skv_record_cache* cache, const skv_record_cache* to, int kee
   a.to_positions = cache->positions ? to->positions : nullptr;
   a.to_weights = to->weights;
   a.to_lengths = to->lengths;
+  a.to_status = to->status;
   a.keep = keep;
   a.sink = sink;
   a.local = local;

@@ -365,14 +365,17 @@ __global__ __launch_bounds__(EV_COPY) void k_evict_copy(EvictArgs a, const int* 
     const uint4 x = reinterpret_cast<const uint4*>(a.from.records + from * 512)[lane];
     const float w = a.weights[slot];
     const int p = a.to_positions ? a.positions[slot] : 0;
+    if (a.to.table) {
+      const uint32_t page = a.to.page(b, i);
+      if (page >= a.to.n_pages) {  // dropped
+        if (lane == 0 && a.to_status) atomicOr(a.to_status, STATUS_PAGE);
+        continue;
+      }
+      to = a.to.row_in(page, g, i);
+    }
     if (lane == 0) {
       if (a.to_weights) a.to_weights[to_slot] = w;
       if (a.to_positions) a.to_positions[to_slot] = p;
-    }
-    if (a.to.table) {
-      const uint32_t page = a.to.page(b, i);
-      if (page >= a.to.n_pages) continue;
-      to = a.to.row_in(page, g, i);
     }
     reinterpret_cast<uint4*>(a.to.records + to * 512)[lane] = x;
   }

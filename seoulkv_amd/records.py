@@ -330,7 +330,9 @@ class RecordCache:
         heaviest by ``weights`` (ties: the lowest slot; NaN counts least).
         Slots whose page is none hold no key: they are passed over and count
         nowhere.  Records, positions and weights go along and ``to.lengths``
-        is set; this cache does not change.  Heads keep different tokens:
+        is set; this cache does not change.  What falls on a slot of ``to``
+        without a page is dropped and reported by ``to.synchronize()``.  Heads
+        keep different tokens:
         ``to.positions`` says which (needs positions in both caches)."""
         if not isinstance(to, RecordCache):
             raise TypeError("expected a RecordCache to evict into")
@@ -352,8 +354,9 @@ class RecordCache:
         _hip.call_on(self._index, "skv_evict", desc, to_desc, keep, sink, local, work.data_ptr(), size)
 
     def synchronize(self) -> None:
-        """Wait for the device; raise if a write since the last call dropped
-        tokens (past the capacity, or without a page)."""
+        """Wait for the device; raise if a write or an eviction into this cache
+        since the last call dropped tokens (past the capacity, or without a
+        page)."""
         torch.cuda.synchronize(self.device)
         bits = int(self.status.item())
         if bits:

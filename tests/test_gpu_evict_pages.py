@@ -108,3 +108,16 @@ def test_captured_evictions_follow_the_table():
         check_eviction(cache, 64, 4, 8, eager)
         assert torch.equal(small.records, eager.records) and torch.equal(small.positions, eager.positions)
         assert torch.equal(small.weights, eager.weights) and torch.equal(small.lengths, eager.lengths)
+
+
+@pytest.mark.parametrize("length", [200, 40000])
+def test_what_falls_on_no_page_is_dropped_and_reported(length):
+    cache = make([length, 90], length, seed=59)
+    to = make([0, 0], 96, 16, seed=61)
+    holes(to, (0, 1), (0, 5), (1, 0))
+    check_eviction(cache, 96, 8, 8, to)
+    cache.synchronize()
+    with pytest.raises(RuntimeError, match="without a page"):
+        to.synchronize()
+    to.synchronize()  # said once
+    verify(to, queries(2, 2), torch.zeros(2, 2, dtype=torch.int64, device=DEV))
