@@ -299,7 +299,8 @@ int skv_rotary(const skv_rotary_table *table, const skv_rows *x, const skv_rows 
  * the turned K as FP8 records (one rounding from FP32), the position and a
  * zero weight where the cache has those arrays (a position's low 32 bits).  k, v: BF16 rows [batch][n][4]
  * [256].  table NULL: K is stored as given.  q (NULL: none): BF16 rows
- * [batch][n][16][256], turned like K into q_out, BF16 rows that may be q.
+ * [batch][n][16][256], turned like K into q_out, BF16 rows that may be q and
+ * share no element with k or v (they may be other heads of the same rows).
  * positions NULL: token i of sequence b has position lengths[b] + i; else
  * device [batch][n], int32 or int64.  counts NULL: n tokens each; else device
  * [batch], tokens i >= counts[b] are not written (their q_out is still

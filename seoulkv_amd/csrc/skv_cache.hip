@@ -3,6 +3,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <numeric>
 
 #include "../../include/seoulkv4_hip.h"
 #include "skv_cache.h"
@@ -68,6 +69,39 @@ bool rows_apart(const Rows& r, int batch, int n, int heads, int dim) {
 bool overlap(const void* a, uint64_t na, const void* b, uint64_t nb) {
   const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
   return a && b && x < y + nb && y < x + na;
+}
+
+// Whether two row tensors of `batch` x n tokens share no byte, by strides alone:
+// for some of the dimensions, both step along these in multiples of a period,
+// and what y spans along the others lies between what x does and its copy a
+// period on (heads of one fused row: the token's stride).  No such dimensions:
+// may overlap.
+bool apart(const Rows& x, int x_heads, const Rows& y, int y_heads, int batch, int n, int dim, unsigned size) {
+  const int64_t x_stride[3] = {x.sb, x.st, x.sh}, y_stride[3] = {y.sb, y.st, y.sh};
+  const int x_count[3] = {batch, n, x_heads}, y_count[3] = {batch, n, y_heads};
+  for (int steps = 0; steps < 8; ++steps) {
+    uint64_t period = 0, x_span = dim, y_span = dim;
+    auto add = [&](int d, int count, int64_t stride, uint64_t& span) {
+      if (count == 1) return;
+      if (steps >> d & 1) period = std::gcd(period, (uint64_t)stride);
+      else span += (uint64_t)(count - 1) * stride;
+    };
+    for (int d = 0; d < 3; ++d) {
+      add(d, x_count[d], x_stride[d], x_span);
+      add(d, y_count[d], y_stride[d], y_span);
+    }
+    x_span *= size;
+    y_span *= size;
+    if (period == 0) {
+      if (!overlap(x.data, x_span, y.data, y_span)) return true;
+      continue;
+    }
+    period *= size;
+    const int64_t off = (int64_t)((uintptr_t)y.data - (uintptr_t)x.data) % (int64_t)period;
+    const uint64_t from = off < 0 ? off + period : off;
+    if (x_span <= from && from + y_span <= period) return true;
+  }
+  return false;
 }
 
 Rows rows_of(Check& c, const char* name, const skv_rows* r, int batch, int n, int heads, int dim,
@@ -227,12 +261,10 @@ int skv_cache_write(const skv_record_cache* cache, const skv_rotary_table* table
     a.q = rows_of(c, "q", q, batch, n, QHEADS, SKV_DIM, 2, false);
     if (c.ok()) a.q_out = rows_of(c, "q_out", q_out, batch, n, QHEADS, SKV_DIM, 2, true);
     if (c.ok()) in_place_or_apart(c, "q_out", a.q, a.q_out, batch, n, QHEADS, SKV_DIM, 2);
-    const uint64_t bytes = extent(a.q_out, batch, n, QHEADS, SKV_DIM) * 2;
-    // k and v are read while q_out is written: they may share its buffer only
-    // as other heads of one row, in place
-    if (c.ok() && a.q.data != a.q_out.data)
-      c.require(!overlap(a.q_out.data, bytes, a.k.data, extent(a.k, batch, n, GROUPS, SKV_DIM) * 2) &&
-                    !overlap(a.q_out.data, bytes, a.v.data, extent(a.v, batch, n, GROUPS, SKV_DIM) * 2),
+    // k and v are read while q_out is written
+    if (c.ok())
+      c.require(apart(a.q_out, QHEADS, a.k, GROUPS, batch, n, SKV_DIM, 2) &&
+                    apart(a.q_out, QHEADS, a.v, GROUPS, batch, n, SKV_DIM, 2),
                 "q_out overlaps k or v");
   }
   if (c.ok() && counts) c.memory("counts", counts, (uint64_t)batch * 4, 4);

@@ -1,0 +1,58 @@
+/* Drives the checks of the record cache's entry points on how row tensors lie
+ * to each other, over the stub of records_stub_driver.c.
+ * tests/test_records_rows.py builds and runs it. */
+int stub_main(void);
+#define main stub_main
+#include "records_stub_driver.c"
+#undef main
+
+static skv_rows at(size_t base, int64_t sb, int64_t st, int64_t sh) {
+  skv_rows r = {arena + base, sb, st, sh};
+  return r;
+}
+
+int main(void) {
+  arena = aligned_alloc(4096, ARENA);
+  if (!arena) return 3;
+  skv_record_cache c = cache();
+  const skv_rotary_table t = {(const uint64_t *)(arena + (20 << 20)), 128, 0, 1.0f};
+  const size_t M = 8 << 20;
+#define PUT(K, V, Q, O, N) skv_cache_write(&c, &t, &K, &V, &Q, &O, N, NULL, 0, NULL, NULL)
+
+  /* 3 tokens of 2 sequences, 24 heads a token (16 of q, 4 of k, 4 of v) */
+  const int64_t st = 24 * 256, sb = 3 * st;
+  const skv_rows q = at(M, sb, st, 256), k = at(M + 16 * 512, sb, st, 256), v = at(M + 20 * 512, sb, st, 256);
+  const skv_rows last_of_q = at(M + 12 * 512, sb, st, 256), one_over = at(M + 15 * 512, sb, st, 256);
+  const skv_rows before = at(M + 3 * 512, sb, st, 256), later = at(M + 4 * 2 * st, sb, st, 256);
+  accept("fused rows in place", PUT(k, v, q, q, 3));
+  accept("one token", PUT(k, v, q, q, 1));
+  refuse("k in q", PUT(last_of_q, v, q, q, 3), "overlaps k or v");
+  refuse("v in q", PUT(k, before, q, q, 3), "overlaps k or v");
+  refuse("one head of k in q", PUT(one_over, v, q, q, 3), "overlaps k or v");
+  refuse("k is q", PUT(q, v, q, q, 3), "overlaps k or v");
+  refuse("k in another token's q", PUT(later, v, q, q, 3), "overlaps k or v");
+  refuse("k in q, one token", PUT(one_over, v, q, q, 1), "overlaps k or v");
+
+  /* heads before tokens */
+  const int64_t hs = 3 * 256, hb = 24 * hs;
+  const skv_rows hq = at(M, hb, 256, hs), hk = at(M + 16 * 2 * hs, hb, 256, hs), hv = at(M + 20 * 2 * hs, hb, 256, hs);
+  const skv_rows hin = at(M + 15 * 2 * hs, hb, 256, hs);
+  accept("heads first in place", PUT(hk, hv, hq, hq, 3));
+  refuse("heads first, k in q", PUT(hin, hv, hq, hq, 3), "overlaps k or v");
+
+  /* broadcast k and v, every other head of a row */
+  const skv_rows bk = at(2 * M, 0, 0, 256), bv = at(2 * M + 2048, 0, 0, 0);
+  accept("broadcast k and v", PUT(bk, bv, q, q, 3));
+  const skv_rows even = at(M, 2 * 3 * 32 * 256, 32 * 256, 512), odd = at(M + 512, 2 * 3 * 32 * 256, 32 * 256, 512);
+  accept("k between the heads of q", PUT(odd, bv, even, even, 3));
+  const skv_rows part = at(M + 2, 2 * 3 * 32 * 256, 32 * 256, 512);
+  refuse("k one element into q", PUT(part, bv, even, even, 3), "overlaps k or v");
+
+  /* turned into another place of the fused rows */
+  const skv_rows from = at(3 * M, 3 * 16 * 256, 16 * 256, 256);
+  accept("q turned into the rows beside k and v", PUT(k, v, from, q, 3));
+  refuse("q turned over k", PUT(one_over, v, from, q, 3), "overlaps k or v");
+
+  printf("records rows driver ok: %d checks\n", checks);
+  return 0;
+}
