@@ -290,7 +290,7 @@ enum { SKV_BF16 = 0, SKV_FP16 = 1, SKV_FP32 = 2 };
  * y).  FP32 arithmetic from 64-bit angles, one rounding to dtype.  dim <=
  * 1024; positions: device [n] (position_batch_stride 0) or [batch] rows of n
  * at that stride, int32 or int64.  y may be x with the same strides;
- * otherwise they must not overlap. */
+ * otherwise they share no element (they may be other heads of the same rows). */
 int skv_rotary(const skv_rotary_table *table, const skv_rows *x, const skv_rows *y, int dtype,
                int batch, int n, int heads, int dim, const void *positions,
                int64_t position_batch_stride, int positions64, int transpose, void *stream);

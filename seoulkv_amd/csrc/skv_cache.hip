@@ -126,8 +126,7 @@ void in_place_or_apart(Check& c, const char* name, const Rows& x, const Rows& y,
                        int heads, int dim, unsigned size) {
   const bool same = x.data == y.data && (batch == 1 || x.sb == y.sb) && (n == 1 || x.st == y.st) &&
                     (heads == 1 || x.sh == y.sh);
-  c.require(same || !overlap(x.data, extent(x, batch, n, heads, dim) * size, y.data,
-                             extent(y, batch, n, heads, dim) * size),
+  c.require(same || apart(x, heads, y, heads, batch, n, dim, size),
             "%s overlaps its input in another layout", name);
 }
 

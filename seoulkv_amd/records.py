@@ -231,7 +231,7 @@ class RecordCache:
         FP8; the slots' positions are set and their weights zeroed.  ``k``,
         ``v``: BF16 [batch, n, 4, 256], any strides with a contiguous last
         dimension.  ``q`` (BF16 [batch, n, 16, 256]) is turned likewise and
-        returned (in ``q_out`` if given, which may be ``q``).  ``counts``
+        returned (in ``q_out`` if given, which may be ``q``; not over ``k`` or ``v``).  ``counts``
         (int32 [batch]): only the first ``counts[b]`` tokens are stored.
         Tokens past the capacity are dropped and reported by
         :meth:`synchronize`.  ``lengths`` does not change."""

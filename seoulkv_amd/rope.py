@@ -126,7 +126,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, table: RotaryTable, *,
     last dimension contiguous, other strides free, e.g. the query and key heads
     of a fused projection) turned to ``positions`` (int32 or int64, [n] or
     [batch, n], any sign).  ``out``: a tensor like ``x`` to write, which may
-    be ``x`` itself; else a new contiguous one.  ``transpose`` applies the
+    be ``x`` itself or other heads of its rows; else a new contiguous one.  ``transpose`` applies the
     transposed map: given the gradient with respect to the result it returns
     the gradient with respect to ``x`` (and, for scale 1, undoes the turn).
     Enqueued on PyTorch's current stream; FP32 arithmetic, rounded once."""

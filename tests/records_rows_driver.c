@@ -53,6 +53,21 @@ int main(void) {
   accept("q turned into the rows beside k and v", PUT(k, v, from, q, 3));
   refuse("q turned over k", PUT(one_over, v, from, q, 3), "overlaps k or v");
 
+  /* rotary: heads beside heads, token rows beside token rows */
+  const skv_rotary_table small = {t.turns, 32, 1, 1.0f};
+#undef TURN
+#define TURN(X, Y, B, N, H) skv_rotary(&small, &X, &Y, SKV_BF16, B, N, H, 256, positions, 0, 1, 0, NULL)
+  int64_t *positions = (int64_t *)(arena + (23 << 20));
+  const skv_rows heads = at(M, sb, st, 256), beside = at(M + 4 * 512, sb, st, 256), over = at(M + 3 * 512, sb, st, 256);
+  accept("heads beside heads", TURN(heads, beside, 2, 3, 4));
+  accept("one token's heads beside its heads", TURN(heads, beside, 1, 1, 4));
+  refuse("heads over heads", TURN(heads, over, 2, 3, 4), "overlaps its input");
+  const skv_rows first = at(M, 0, 2 * 1024, 256), second = at(M + 2048, 0, 2 * 1024, 256);
+  accept("every other token", TURN(first, second, 1, 5, 4));
+  refuse("every other token, 5 heads", TURN(first, second, 1, 5, 5), "overlaps its input");
+  const skv_rows wide = at(M, sb, st, 256), narrow = at(M, sb, st, 512);
+  refuse("the same start in another layout", TURN(wide, narrow, 2, 3, 4), "overlaps its input");
+
   printf("records rows driver ok: %d checks\n", checks);
   return 0;
 }
