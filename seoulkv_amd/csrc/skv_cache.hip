@@ -47,6 +47,12 @@ struct Check {
   int device_ = -1;
 };
 
+// Whether `count` steps of a stride reach at most 2^40 elements, which keeps
+// every sum and product below in 64 bits.
+bool steps_fit(int64_t stride, int count) {
+  return stride >= 0 && stride <= ((int64_t)1 << 40) / (count > 1 ? count - 1 : 1);
+}
+
 // Elements from a row tensor's first to one past its last.
 uint64_t extent(const Rows& r, int batch, int n, int heads, int dim) {
   return (uint64_t)(batch - 1) * r.sb + (uint64_t)(n - 1) * r.st + (uint64_t)(heads - 1) * r.sh + dim;
@@ -110,10 +116,8 @@ Rows rows_of(Check& c, const char* name, const skv_rows* r, int batch, int n, in
   if (!c.ok()) return out;
   if (!c.require(r != nullptr, "NULL %s rows", name)) return out;
   out = Rows{r->data, r->batch_stride, r->token_stride, r->head_stride};
-  // 2^40 elements per stride keep every product below in 64 bits
-  constexpr int64_t MOST = (int64_t)1 << 40;
-  if (!c.require(out.sb >= 0 && out.st >= 0 && out.sh >= 0 && out.sb <= MOST && out.st <= MOST &&
-                     out.sh <= MOST, "%s: strides must lie in [0, 2^40]", name))
+  if (!c.require(steps_fit(out.sb, batch) && steps_fit(out.st, n) && steps_fit(out.sh, heads),
+                 "%s: strides must lie in [0, 2^40], their steps in all too", name))
     return out;
   if (output && !c.require(rows_apart(out, batch, n, heads, dim), "%s: output rows overlap", name))
     return out;
@@ -188,7 +192,7 @@ RotaryArgs rotary_of(Check& k, const skv_rotary_table* t, const void* positions,
     r.pairs = t->pairs;
     r.scale = t->scale;
   }
-  if (positions && k.require(sb == 0 || sb >= n, "position rows of %d at stride %lld", n, (long long)sb)) {
+  if (positions && k.require((sb == 0 || sb >= n) && steps_fit(sb, batch), "position rows of %d at stride %lld", n, (long long)sb)) {
     const unsigned size = positions64 ? 8 : 4;
     k.memory("positions", positions, ((uint64_t)(batch - 1) * sb + n) * size, size);
   }

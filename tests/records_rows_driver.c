@@ -68,6 +68,19 @@ int main(void) {
   const skv_rows wide = at(M, sb, st, 256), narrow = at(M, sb, st, 512);
   refuse("the same start in another layout", TURN(wide, narrow, 2, 3, 4), "overlaps its input");
 
+  /* strides whose reach wraps round 64 bits */
+  const skv_rotary_table one = {t.turns, 1, 0, 1.0f};
+  const int many = (1 << 25) + 1; /* times 2^39 elements */
+  const skv_rows far_in = at(M, (int64_t)1 << 39, 2, 2), flat = at(3 * M, 2, 2, 2), all_one = at(3 * M, 0, 2, 2);
+#define FAR(X, Y, B, N, P, SB) skv_rotary(&one, &X, &Y, SKV_BF16, B, N, 1, 2, P, SB, 1, 0, NULL)
+  refuse("x and y wrap round", FAR(far_in, far_in, many, 1, positions, 0), "strides");
+  refuse("y wraps round", FAR(all_one, far_in, many, 1, positions, 0), "strides");
+  const skv_rows far_tokens = at(M, 0, (int64_t)1 << 39, 2);
+  refuse("tokens wrap round", FAR(far_tokens, flat, 1, many, positions, 0), "");
+  refuse("positions wrap round", FAR(flat, flat, 5, 1, positions, (int64_t)1 << 62), "position rows");
+  refuse("positions wrap round in bytes", FAR(flat, flat, 5, 1, positions, (int64_t)1 << 59), "position rows");
+  refuse("positions before their start", FAR(flat, flat, 5, 1, positions, -8), "position rows");
+
   printf("records rows driver ok: %d checks\n", checks);
   return 0;
 }
