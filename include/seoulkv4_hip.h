@@ -302,7 +302,7 @@ int skv_rotary(const skv_rotary_table *table, const skv_rows *x, const skv_rows 
  * [batch][n][16][256], turned like K into q_out, BF16 rows that may be q and
  * share no element with k or v (they may be other heads of the same rows).
  * positions NULL: token i of sequence b has position lengths[b] + i; else
- * device [batch][n], int32 or int64.  counts NULL: n tokens each; else device
+ * device [batch][n], int32 or int64, outside the cache's own.  counts NULL: n tokens each; else device
  * [batch], tokens i >= counts[b] are not written (their q_out is still
  * defined).  lengths does not change: tokens are drafts until the caller
  * raises it. */

@@ -257,6 +257,10 @@ int skv_cache_write(const skv_record_cache* cache, const skv_rotary_table* table
   c.require((q == nullptr) == (q_out == nullptr), "q and q_out go together");
   if (!c.ok()) return c.code;
   a.r = rotary_of(c, table, positions, n, positions64, batch, n, SKV_DIM);
+  if (c.ok())
+    c.require(!overlap(positions, (uint64_t)batch * n * (positions64 ? 8 : 4), cache->positions,
+                       (uint64_t)batch * GROUPS * cache->capacity * 4),
+              "the positions lie in the cache's own, which the write changes");
   a.interleaved = table ? table->interleaved != 0 : 0;
   if (c.ok()) a.k = rows_of(c, "k", k, batch, n, GROUPS, SKV_DIM, 2, false);
   if (c.ok()) a.v = rows_of(c, "v", v, batch, n, GROUPS, SKV_DIM, 2, false);

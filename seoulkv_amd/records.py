@@ -257,6 +257,9 @@ class RecordCache:
                                   or table.rotary_dim > HEAD_DIM):
             raise ValueError(f"expected a RotaryTable of at most {HEAD_DIM} elements on {self.device}")
         positions = self._optional("positions", positions, (torch.int32, torch.int64), (self.batch, n))
+        if positions is not None and self.positions is not None and \
+                positions.untyped_storage().data_ptr() == self.positions.untyped_storage().data_ptr():
+            positions = positions.clone()  # slots' own positions change while they are read
         counts = self._optional("counts", counts, (torch.int32,), (self.batch,))
         _no_grad("write", k, v, q)
         if n == 0:

@@ -81,6 +81,17 @@ int main(void) {
   refuse("positions wrap round in bytes", FAR(flat, flat, 5, 1, positions, (int64_t)1 << 59), "position rows");
   refuse("positions before their start", FAR(flat, flat, 5, 1, positions, -8), "position rows");
 
+  /* positions that the write itself changes */
+#define AT(C, P, WIDE) skv_cache_write(&C, &t, &k, &v, NULL, NULL, 3, P, WIDE, NULL, NULL)
+  accept("positions of their own", AT(c, positions, 1));
+  refuse("the cache's positions", AT(c, c.positions + 64, 0), "cache's own");
+  refuse("into the cache's positions", AT(c, c.positions - 5, 0), "cache's own");
+  refuse("64-bit ones there", AT(c, c.positions + 2 * 4 * 64 - 2, 1), "cache's own");
+  accept("behind them", AT(c, c.positions + 2 * 4 * 64, 0));
+  skv_record_cache plain = c;
+  plain.positions = NULL;
+  accept("a cache without", AT(plain, c.positions + 64, 0));
+
   printf("records rows driver ok: %d checks\n", checks);
   return 0;
 }

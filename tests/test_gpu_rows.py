@@ -45,3 +45,14 @@ def test_queries_turned_beside_the_keys_and_values_of_their_rows():
                          (inside, v, q, rows[:, :, :16])):
         with pytest.raises(ValueError, match="overlaps k or v"):
             cache.write(k, v, q=q, table=table, q_out=out)
+
+
+def test_positions_that_the_write_itself_changes():
+    """Slots' own positions as the new ones: read before any is stored."""
+    cache, other = make([100], 640), make([100], 640)
+    k, v = (torch.randn(1, 256, 4, 256, generator=gen(s)).bfloat16().to(DEV) for s in (1, 2))
+    table = RotaryTable(256, base=1e6, device=DEV)
+    own = cache.positions[:, 0, 20:276]  # slots 100 .. 275 of it are written
+    other.write(k, v, table=table, positions=own.clone())
+    cache.write(k, v, table=table, positions=own)
+    assert torch.equal(cache.positions, other.positions) and torch.equal(cache.records, other.records)
