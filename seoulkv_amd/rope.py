@@ -23,6 +23,7 @@ import math
 from fractions import Fraction
 
 import torch
+from torch.autograd import forward_ad
 
 from seoulkv_amd import _hip
 
@@ -118,6 +119,10 @@ class RotaryTable:
 def _no_grad(name: str, *tensors) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise ValueError(f"{name} records no gradients: call it under torch.no_grad()")
+    # (forward mode goes on under no_grad; -1 outside every dual_level)
+    if forward_ad._current_level >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError(f"{name} records no forward gradients: give it the primal alone")
 
 
 def rotary(x: torch.Tensor, positions: torch.Tensor, table: RotaryTable, *,
