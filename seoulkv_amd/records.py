@@ -261,7 +261,7 @@ class RecordCache:
                 positions.untyped_storage().data_ptr() == self.positions.untyped_storage().data_ptr():
             positions = positions.clone()  # slots' own positions change while they are read
         counts = self._optional("counts", counts, (torch.int32,), (self.batch,))
-        _no_grad("write", k, v, q)
+        _no_grad("write", k, v, q, q_out, self.weights)
         if n == 0:
             return q_out
         _hip.call_on(self._index, "skv_cache_write", desc, None if table is None else table._desc,
@@ -287,7 +287,7 @@ class RecordCache:
         n = q.shape[1]
         tree = self._optional("tree", tree, (torch.int64,), (self.batch, n))
         counts = self._optional("counts", counts, (torch.int32,), (self.batch,))
-        _no_grad("tree_decode", q)
+        _no_grad("tree_decode", q, out, lse)
         if out is None:
             out = q.new_empty((self.batch, n, N_HEADS, HEAD_DIM))
         elif not out.is_contiguous() or self._rows("out", out, N_HEADS).shape[1] != n:
@@ -320,7 +320,7 @@ class RecordCache:
         lse = self._optional("lse", lse, (torch.float32,), (self.batch, n, N_HEADS))
         if lse is None:
             raise ValueError("key_weights needs tree_decode's lse")
-        _no_grad("key_weights", q, lse)
+        _no_grad("key_weights", q, lse, self.weights)
         if n == 0:
             raise ValueError("key_weights needs at least one row")
         _hip.call_on(self._index, "skv_key_weights", desc, _hip.rows_desc(q), n, lse.data_ptr(),
@@ -349,6 +349,7 @@ class RecordCache:
             raise ValueError(f"keep {keep} must hold sink {sink} + local {local} and fit the capacity "
                              f"{to.capacity}")
         to._writable()
+        _no_grad("evict", self.weights, to.weights)
         if self._pages is not None and to._pages is not None and \
                 self.records.data_ptr() == to.records.data_ptr() and not self._pages.isdisjoint(to._pages):
             raise ValueError("the two caches share pages")

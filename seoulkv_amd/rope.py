@@ -146,7 +146,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, table: RotaryTable, *,
         raise ValueError("expected int32 or int64 positions [n] or [batch, n]")
     if not x.device == positions.device == table.device:
         raise ValueError("x, positions and table must be on one device")
-    _no_grad("rotary", x)
+    _no_grad("rotary", x, out)
     if out is None:
         out = x.new_empty(shape)
     elif out.shape != shape or out.dtype != x.dtype or out.device != x.device:

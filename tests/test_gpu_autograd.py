@@ -41,3 +41,27 @@ def test_forward_mode_is_refused():
                 call()
         rotary(x, positions, table)  # nothing of theirs is dual
         cache.write(k, v, q=q)
+
+
+def test_outputs_that_ask_for_gradients_are_refused():
+    x, positions, table = setup_rows()
+    cache, q = make([40, 7], 64), queries(2, 3)
+    k, v = kv()
+    out, lse = cache.tree_decode(q)
+    small = RecordCache.allocate(2, 32, device=DEV)
+    weights = torch.zeros(2, 4, 64, device=DEV, requires_grad=True)
+    asking = RecordCache(cache.records, cache.lengths, weights=weights)
+    calls = (lambda: rotary(x, positions, table, out=torch.zeros_like(x).requires_grad_()),
+             lambda: cache.tree_decode(q, out=torch.zeros_like(out).requires_grad_()),
+             lambda: cache.tree_decode(q, lse=torch.zeros_like(lse).requires_grad_()),
+             lambda: cache.write(k, v, q=q, q_out=torch.zeros_like(q).requires_grad_()),
+             lambda: asking.write(k, v), lambda: asking.key_weights(q, lse),
+             lambda: asking.evict(small, 8, sink=1, local=1),
+             lambda: cache.evict(RecordCache(small.records, small.lengths, weights=torch.zeros(
+                 2, 4, 32, device=DEV, requires_grad=True)), 8, sink=1, local=1))
+    for i, call in enumerate(calls):
+        with pytest.raises(ValueError, match="gradients"):
+            call()
+            pytest.fail(f"call {i} was taken")
+        with torch.no_grad():
+            call()
