@@ -36,7 +36,7 @@ import torch
 
 from seoulkv_amd import _hip
 from seoulkv_amd.paged import KVPagePool, N_KV_HEADS, RECORD_BYTES
-from seoulkv_amd.rope import RotaryTable, _no_grad
+from seoulkv_amd.rope import RotaryTable, _no_grad, _written
 
 N_HEADS, HEAD_DIM = 16, 256
 MAX_DRAFTS = 64
@@ -268,6 +268,7 @@ class RecordCache:
                      _hip.rows_desc(k), _hip.rows_desc(v), None if q is None else _hip.rows_desc(q),
                      None if q is None else _hip.rows_desc(q_out), n, _hip.pointer(positions),
                      positions is not None and positions.dtype == torch.int64, _hip.pointer(counts))
+        _written(self.records, self.positions, self.weights, q_out)
         return q_out
 
     def tree_decode(self, q: torch.Tensor, tree: torch.Tensor | None = None, *,
@@ -288,6 +289,7 @@ class RecordCache:
         tree = self._optional("tree", tree, (torch.int64,), (self.batch, n))
         counts = self._optional("counts", counts, (torch.int32,), (self.batch,))
         _no_grad("tree_decode", q, out, lse)
+        given = out, lse
         if out is None:
             out = q.new_empty((self.batch, n, N_HEADS, HEAD_DIM))
         elif not out.is_contiguous() or self._rows("out", out, N_HEADS).shape[1] != n:
@@ -302,6 +304,7 @@ class RecordCache:
         work = q.new_empty(size, dtype=torch.uint8)
         _hip.call_on(self._index, "skv_tree_decode", desc, _hip.rows_desc(q), n, _hip.pointer(tree),
                      _hip.pointer(counts), cap, out.data_ptr(), lse.data_ptr(), work.data_ptr(), size)
+        _written(*given)
         return out, lse
 
     def key_weights(self, q: torch.Tensor, lse: torch.Tensor, tree: torch.Tensor | None = None, *,
@@ -325,6 +328,7 @@ class RecordCache:
             raise ValueError("key_weights needs at least one row")
         _hip.call_on(self._index, "skv_key_weights", desc, _hip.rows_desc(q), n, lse.data_ptr(),
                      _hip.pointer(tree), _hip.pointer(counts), cap, bool(accumulate))
+        _written(self.weights)
 
     def evict(self, to: "RecordCache", keep: int, *, sink: int = 128, local: int = 256) -> None:
         """Copy what stays of every sequence and KV head into ``to`` (same
@@ -356,6 +360,7 @@ class RecordCache:
         size = _hip.load_library().skv_evict_workspace(self.batch, self.capacity, keep)
         work = torch.empty(size, dtype=torch.uint8, device=self.device)
         _hip.call_on(self._index, "skv_evict", desc, to_desc, keep, sink, local, work.data_ptr(), size)
+        _written(to.records, to.positions if self.positions is not None else None, to.weights, to.lengths)
 
     def synchronize(self) -> None:
         """Wait for the device; raise if a write or an eviction into this cache

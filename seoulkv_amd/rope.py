@@ -125,6 +125,14 @@ def _no_grad(name: str, *tensors) -> None:
         raise ValueError(f"{name} records no forward gradients: give it the primal alone")
 
 
+def _written(*tensors) -> None:
+    """Count a change of the caller's tensors that a kernel wrote, for graphs
+    that saved them."""
+    tensors = [t for t in tensors if t is not None]
+    if tensors:
+        torch.autograd.graph.increment_version(tensors)
+
+
 def rotary(x: torch.Tensor, positions: torch.Tensor, table: RotaryTable, *,
            out: torch.Tensor | None = None, transpose: bool = False) -> torch.Tensor:
     """``x`` [n, heads, dim] or [batch, n, heads, dim] (BF16, FP16 or FP32; the
@@ -147,6 +155,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, table: RotaryTable, *,
     if not x.device == positions.device == table.device:
         raise ValueError("x, positions and table must be on one device")
     _no_grad("rotary", x, out)
+    given = out
     if out is None:
         out = x.new_empty(shape)
     elif out.shape != shape or out.dtype != x.dtype or out.device != x.device:
@@ -161,4 +170,5 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, table: RotaryTable, *,
     _hip.call_on(x.device.index, "skv_rotary", table._desc, _hip.rows_desc(x), _hip.rows_desc(out),
                  dtype, batch, x.shape[-3], x.shape[-2], x.shape[-1], positions.data_ptr(), per_batch,
                  positions.dtype == torch.int64, bool(transpose))
+    _written(given)
     return out

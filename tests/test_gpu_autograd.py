@@ -65,3 +65,31 @@ def test_outputs_that_ask_for_gradients_are_refused():
             pytest.fail(f"call {i} was taken")
         with torch.no_grad():
             call()
+
+
+def test_changed_tensors_are_marked_for_a_graph_that_saved_them():
+    x, positions, table = setup_rows()
+    cache, q = make([40, 7], 64), queries(2, 3)
+    k, v = kv()
+    small = RecordCache.allocate(2, 32, device=DEV)
+    out, lse = cache.tree_decode(q)
+    y, turned = torch.zeros_like(x), torch.zeros_like(q)
+    cases = [(lambda: rotary(x, positions, table, out=y), (y,)), (lambda: rotary(x, positions, table, out=x), (x,)),
+             (lambda: cache.write(k, v, q=q, q_out=turned), (cache.records, cache.positions, cache.weights, turned)),
+             (lambda: cache.tree_decode(q, out=out, lse=lse), (out, lse)),
+             (lambda: cache.key_weights(q, lse), (cache.weights,)),
+             (lambda: cache.evict(small, 8, sink=1, local=1),
+              (small.records, small.positions, small.weights, small.lengths))]
+    every = [t for _, written in cases for t in written] + [q, k, v, cache.lengths, positions]
+    for i, (call, written) in enumerate(cases):
+        before = [t._version for t in every]
+        call()
+        for t, version in zip(every, before):
+            assert (t._version > version) == any(t is w for w in written), (i, t.shape)
+    factor = torch.ones_like(lse, requires_grad=True)
+    loss = (factor * lse).sum()
+    cache.tree_decode(q, out=out, lse=lse)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():  # tensors without a counter
+        cache.tree_decode(q, out=torch.empty_like(out))
