@@ -108,7 +108,7 @@ TRACE_LIB_PATH = LIB_PATH.with_name("libseoulkv4_hip_trace.so")
 
 _lib = None
 _trace_lib = None
-_raw_stream = torch._C._cuda_getCurrentRawStream
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # none: a PyTorch without GPUs
 
 
 def load_library() -> ctypes.CDLL:
