@@ -18,12 +18,13 @@ One round of speculative decoding::
 
     q = cache.write(k, v, q=q, table=table, positions=pos)   # drafts, rotated
     out, lse = cache.tree_decode(q, tree)                     # verify them
+    cache.key_weights(q, lse, tree)                           # on the steps that count
     ...                                                       # accept some
-    cache.write(k_accepted, v_accepted, table=table)          # store the path
+    cache.write(k_accepted, v_accepted, table=table, positions=pos_accepted)
     cache.lengths += accepted
 
-and, when a cache has grown to its budget, ``cache.key_weights(q, lse)`` on the
-steps that count and ``cache.evict(smaller, keep)``.
+and, when a cache has grown to its budget, ``cache.evict(smaller, keep)``.
+``lengths`` counts slots: after an eviction it is no position any more.
 
 All calls enqueue on PyTorch's current stream and never synchronise; tensors
 used on another stream are the caller's to order, as with any torch operator.
@@ -227,8 +228,8 @@ class RecordCache:
               counts: torch.Tensor | None = None, q_out: torch.Tensor | None = None) -> torch.Tensor | None:
         """Store n tokens of every sequence in slots ``lengths[b] ..``: V, and
         K turned by ``table`` (``None``: as given) to ``positions`` (int32 or
-        int64 [batch, n]; default ``lengths[b] + i``), each rounded once to
-        FP8; the slots' positions are set and their weights zeroed.  ``k``,
+        int64 [batch, n]; default ``lengths[b] + i``, which is right as long as
+        slots are positions: not after an eviction), each rounded once to FP8; the slots' positions are set and their weights zeroed.  ``k``,
         ``v``: BF16 [batch, n, 4, 256], any strides with a contiguous last
         dimension.  ``q`` (BF16 [batch, n, 16, 256]) is turned likewise and
         returned (in ``q_out`` if given, which may be ``q``; not over ``k`` or ``v``).  ``counts``
@@ -312,7 +313,9 @@ class RecordCache:
         """Add to ``weights[b][g][t]`` the attention weight exp(score - lse)
         that the rows of :meth:`tree_decode` (same arguments; ``lse``: its
         result) and the 4 query heads of KV head g give slot t; with
-        ``accumulate=False`` replace it (slots past the drafts stay)."""
+        ``accumulate=False`` replace it (slots past the drafts stay).  The
+        cache has to be as it was then: ``lse`` belongs to those lengths and
+        records."""
         desc = self._open()
         if self.weights is None:
             raise ValueError("the cache has no weights")
@@ -339,8 +342,8 @@ class RecordCache:
         nowhere.  Records, positions and weights go along and ``to.lengths``
         is set; this cache does not change.  What falls on a slot of ``to``
         without a page is dropped and reported by ``to.synchronize()``.  Heads
-        keep different tokens:
-        ``to.positions`` says which (needs positions in both caches)."""
+        keep different tokens: ``to.positions`` says which (needs positions in
+        both caches); the position after the last is not ``to.lengths``."""
         if not isinstance(to, RecordCache):
             raise TypeError("expected a RecordCache to evict into")
         desc, to_desc = self._open(), to._open()

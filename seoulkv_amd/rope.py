@@ -78,7 +78,8 @@ def _turns(inv) -> torch.Tensor:
 
 
 class RotaryTable:
-    """Angles per position of a head's pairs, on one device.
+    """Angles per position of a head's pairs, on one device; built once and used
+    for every call (it forms exact fractions on the host and copies them).
 
     ``rotary_dim``: elements that turn (even).  ``inverse_frequencies``: the
     ``rotary_dim / 2`` angles per position in radians, instead of ``base`` and
