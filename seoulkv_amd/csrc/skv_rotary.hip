@@ -29,11 +29,17 @@ __device__ __forceinline__ int64_t position_of(const RotaryArgs& r, int b, int i
                        : static_cast<const int32_t*>(r.positions)[at];
 }
 
-// scale (cos, sin) of `turns` 2^-64 turns per position at position p.
+// scale (cos, sin) of `turns` 2^-64 turns per position at position p.  The
+// angle is brought within an eighth of a turn of a quarter's multiple before it
+// becomes FP32: off by pi 2^-27 then, a whole half turn by pi 2^-25.
 __device__ __forceinline__ float2 turn(uint64_t turns, int64_t p, float scale) {
-  const int hi = (int)((turns * (uint64_t)p) >> 32);
+  const uint32_t hi = (uint32_t)((turns * (uint64_t)p) >> 32);  // 2^-32 turns
+  const uint32_t quarters = (hi + (1u << 29)) >> 30;
   float s, c;
-  sincospif((float)hi * 0x1p-31f, &s, &c);
+  sincospif((float)(int)(hi - (quarters << 30)) * 0x1p-31f, &s, &c);
+  const float a = quarters & 1 ? s : c, b = quarters & 1 ? c : s;
+  c = (quarters + 1) & 2 ? -a : a;
+  s = quarters & 2 ? -b : b;
   return make_float2(c * scale, s * scale);
 }
 
