@@ -3,7 +3,7 @@
 // A pair (a, b) of a head at position p becomes s (a cos t - b sin t, b cos t +
 // a sin t) with t = p inv_i.  inv_i is held in 2^-64 turns, so p inv_i modulo
 // a turn is one wrapping 64-bit product, exact for any position where an FP32
-// angle would be off by p 2^-24 radians; its top 32 bits go to sincospi.
+// angle would be off by p 2^-24 radians; its top 32 bits are the angle.
 //
 // Both kernels are bound by memory.  A thread owns 8 pairs (two 16-byte loads
 // in BF16) of one token and keeps their sines and cosines in registers while
@@ -11,8 +11,13 @@
 // head; few tokens are spread over the chip by splitting the heads.  4 heads
 // are in flight at once.  32768 tokens x 20 heads x 256 in BF16: 139 us, 4.8
 // TB/s (torch's copy of as many bytes: 160 us); 32768 tokens into a cache with
-// their queries: 174 us, 4.2 TB/s (188 with one row in flight); a single
-// token of 8 sequences 4.6 us, the launch.
+// their queries: 173 us, 4.3 TB/s (188 with one row in flight); a single
+// token of 8 sequences 4.4 us, the launch.
+//
+// Where the turned part is no multiple of 16 elements, or rows or strides are
+// not 16-byte aligned, every access is one element (N = 1): 34 of 256 elements
+// of those 32768 x 20 heads 340 us (32 of 256: 226, mostly the copy of what is
+// not turned; in place 34 against 22), written with their queries 404 (32: 181).
 #include "skv_cache.h"
 #include "skv_device.h"
 
@@ -20,6 +25,7 @@ namespace skv {
 
 namespace {
 
+constexpr double PI = 3.14159265358979323846;
 constexpr int RO_BLOCK = 256;
 constexpr int RO_TARGET_BLOCKS = 2048;  // 8 blocks of 4 waves on each of 256 CUs
 
@@ -31,16 +37,30 @@ __device__ __forceinline__ int64_t position_of(const RotaryArgs& r, int b, int i
 
 // scale (cos, sin) of `turns` 2^-64 turns per position at position p.  The
 // angle is brought within an eighth of a turn of a quarter's multiple before it
-// becomes FP32: off by pi 2^-27 then, a whole half turn by pi 2^-25.
+// becomes FP32 (off by pi 2^-27 then, a whole half turn by pi 2^-25), where the
+// series of sin pi r and cos pi r end after r^9 and r^10, within 2e-9 and 2e-10;
+// pi is two words, so a rounding of the sine is one of its last sum.  Off by at
+// most 7.3e-8 in all (4e6 angles), and fewer instructions than a function that
+// reduces its argument once more (5003 x 7 rows of 48 FP32 elements: 8.8 us, 9.4
+// with one).
 __device__ __forceinline__ float2 turn(uint64_t turns, int64_t p, float scale) {
   const uint32_t hi = (uint32_t)((turns * (uint64_t)p) >> 32);  // 2^-32 turns
   const uint32_t quarters = (hi + (1u << 29)) >> 30;
-  float s, c;
-  sincospif((float)(int)(hi - (quarters << 30)) * 0x1p-31f, &s, &c);
+  const float r = (float)(int)(hi << 2) * 0x1p-33f;  // (the low 30 bits, signed)
+  const float t = r * r;
+  constexpr double PI2 = PI * PI;
+  constexpr float PI_HI = (float)PI, PI_LO = (float)(PI - PI_HI);
+  constexpr float S3 = (float)(-PI * PI2 / 6), S5 = (float)(PI * PI2 * PI2 / 120),
+                  S7 = (float)(-PI * PI2 * PI2 * PI2 / 5040), S9 = (float)(PI * PI2 * PI2 * PI2 * PI2 / 362880);
+  constexpr float C2 = (float)(-PI2 / 2), C4 = (float)(PI2 * PI2 / 24), C6 = (float)(-PI2 * PI2 * PI2 / 720),
+                  C8 = (float)(PI2 * PI2 * PI2 * PI2 / 40320),
+                  C10 = (float)(-PI2 * PI2 * PI2 * PI2 * PI2 / 3628800);
+  const float s = fmaf(r, PI_HI, r * fmaf(t, fmaf(t, fmaf(t, fmaf(t, S9, S7), S5), S3), PI_LO));
+  const float c = fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, C10, C8), C6), C4), C2), 1.f);
   const float a = quarters & 1 ? s : c, b = quarters & 1 ? c : s;
-  c = (quarters + 1) & 2 ? -a : a;
-  s = quarters & 2 ? -b : b;
-  return make_float2(c * scale, s * scale);
+  const float cosine = __uint_as_float(__float_as_uint(a) ^ ((quarters + 1) & 2) << 30);
+  const float sine = __uint_as_float(__float_as_uint(b) ^ (quarters & 2) << 30);
+  return make_float2(cosine * scale, sine * scale);
 }
 
 struct BF16 { uint16_t u; };
