@@ -404,6 +404,9 @@ void launch_evict(EvictArgs a, hipStream_t st) {
   a.before_stride = most_pages(a.from.capacity);
   const int middle = a.from.capacity - a.sink - a.local;  // at most; a longer list takes the long path
   if (middle <= EV_ONE) {
+    // as few slots a thread as hold the list (4 lists, whole calls: 4096 slots 16
+    // us, 20 with 16 a thread, 27 with 32, 34 on the long path; 8192: 22, 24, 31,
+    // 38; 16384: 44, 50 with 32, 56; 32768: 54, 56 on the long path)
     auto one = middle <= 4 * EV_BLOCK ? k_evict_one<4> : middle <= 8 * EV_BLOCK ? k_evict_one<8>
                : middle <= 16 * EV_BLOCK ? k_evict_one<16> : k_evict_one<32>;
     hipLaunchKernelGGL(one, dim3(lists), dim3(EV_BLOCK), 0, st, a, kept);

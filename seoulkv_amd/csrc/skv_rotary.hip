@@ -11,7 +11,7 @@
 // head; few tokens are spread over the chip by splitting the heads.  4 heads
 // are in flight at once.  32768 tokens x 20 heads x 256 in BF16: 139 us, 4.8
 // TB/s (torch's copy of as many bytes: 160 us); 32768 tokens into a cache with
-// their queries: 173 us, 4.3 TB/s (188 with one row in flight); a single
+// their queries: 175 us, 4.2 TB/s (188 with one row in flight); a single
 // token of 8 sequences 4.4 us, the launch.
 //
 // Where the turned part is no multiple of 16 elements, or rows or strides are

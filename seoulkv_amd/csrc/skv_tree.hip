@@ -18,13 +18,18 @@
 // a batch of ragged sequences loads every CU alike.  A share that spans
 // sequences leaves one partial in each; k_tree_merge joins a sequence's.
 //
-// Bounds (131072 keys, contiguous, a whole call): one to 4 drafts 49 us, of
-// which the kernel 44, 6.0 TB/s, the record stream; 8 drafts 54, 16 66: the wait
-// for records, since 256 registers a wave leave 8 waves a CU and one pair ahead;
-// 32 drafts 95, 64 drafts 155, with a cap 178: multiplying and weighing, which
-// two waves a SIMD overlap little (loads two or three steps ahead changed
-// nothing there).  Loads pay where no wait stands between their issue and their
-// use: see the loops' notes on branches and spills.
+// Bounds (131072 keys, contiguous, whole calls on one cache over and over): one
+// to 4 drafts 49 us (51 where several caches take turns), of which the kernel
+// 44, 6.0 TB/s, the record stream; 8 drafts 54, 16 66 (73 in turns): the wait for
+// records, since 256 registers a wave leave 8 waves a CU and one pair ahead; 32
+// drafts 93, 64 drafts 154, with a cap 174: multiplying and weighing, which two
+// waves a SIMD overlap little (loads two or three steps ahead changed nothing
+// there).  One draft of many ragged paged sequences: 64 of up to 8192 keys
+// (279530 in all) 113 us, 5.1 TB/s, 256 of up to 4096 (504279) 195 us, 5.3 TB/s:
+// a share holds pieces of several sequences, each with queries to stage and a
+// partial to store.  Loads pay where no wait stands between their issue and
+// their use: see the loops' notes on branches and spills (7 to 9 registers of
+// the two-tile instances are spilled, outside those loops).
 #include <type_traits>
 
 #include "skv_cache.h"
@@ -976,9 +981,10 @@ __global__ __launch_bounds__(SLICES == 1 ? 256 : SLICES * 64) void k_tree_merge(
 // over the rows in registers and then over the 16 lanes of a row group: no
 // atomics, the same bits every time.  Bound by matrix cores, vector units and
 // LDS about alike for many rows, so 4 waves on a SIMD do more than records
-// loaded ahead (32 rows over 131072 keys: 47 us, 70 with 2 waves and a pair
-// ahead); by the K halves, 256 bytes of every 512, for few (one row 29 us a
-// call, 4.6 TB/s).
+// loaded ahead (32 rows over 131072 keys: 46 us, 70 with 2 waves and a pair
+// ahead; 64 rows 67); by the K halves, 256 bytes of every 512, for few (one row
+// 28 us a call, 4.8 TB/s).  4 waves leave 128 registers: 8 are spilled, outside
+// the loop over row tiles.
 // (the 128 KB image of 64 drafts leaves room for one block, of 16 waves then)
 constexpr int weight_waves(int tiles) { return tiles > 8 ? 16 : 8; }
 
@@ -1095,14 +1101,15 @@ template <bool PAGED>
 void tree_rows(const TreeArgs& a, hipStream_t st) {
   const dim3 grid(TR_BLOCKS, G);
   const int tiles = (a.n * H + 15) / 16;
-  // up to 4 drafts: one tile of rows a wave (49 us a call at 131072 keys; 57
-  // with two, the second empty; 62 with 12 waves, whose 168 registers spill)
+  // up to 4 drafts: one tile of rows a wave (49 us a call on one cache of 131072
+  // keys over and over; 57 with two, the second empty; 62 with 12 waves, whose
+  // 168 registers spill)
   if (tiles <= 1) hipLaunchKernelGGL((k_tree<1, 1, 8, PAGED>), grid, dim3(512), 0, st, a);
   // two tiles a wave: widened records serve both (16 drafts 66 us, 99 with
   // one); row waves that hold the same records as far as 16 drafts (12 in 64
   // paged sequences of 2000 keys 72 us, 80 when they are widened once into
-  // LDS), widened once past them (32 drafts 95 us, 122 by 4 row waves each for
-  // itself; 64 drafts 155 us, 219 by 8)
+  // LDS), widened once past them (32 drafts 93 us, 122 by 4 row waves each for
+  // itself; 64 drafts 154 us, 219 by 8)
   else if (tiles <= 2) hipLaunchKernelGGL((k_tree<2, 1, 8, PAGED>), grid, dim3(512), 0, st, a);
   else if (tiles <= 4) hipLaunchKernelGGL((k_tree<2, 2, 4, PAGED>), grid, dim3(512), 0, st, a);
   else if (tiles <= 8) hipLaunchKernelGGL((k_tree_wide<1, PAGED>), grid, dim3(512), 0, st, a);
