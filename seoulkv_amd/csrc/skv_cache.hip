@@ -192,7 +192,8 @@ RotaryArgs rotary_of(Check& k, const skv_rotary_table* t, const void* positions,
     r.pairs = t->pairs;
     r.scale = t->scale;
   }
-  if (positions && k.require((sb == 0 || sb >= n) && steps_fit(sb, batch), "position rows of %d at stride %lld", n, (long long)sb)) {
+  if (positions && k.require((sb == 0 || sb >= n) && steps_fit(sb, batch),
+                             "position rows of %d at stride %lld", n, (long long)sb)) {
     const unsigned size = positions64 ? 8 : 4;
     k.memory("positions", positions, ((uint64_t)(batch - 1) * sb + n) * size, size);
   }

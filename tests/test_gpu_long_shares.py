@@ -169,3 +169,32 @@ def test_not_a_number_in_long_shares(n):
                 want[:] = sees
             assert torch.equal(got, want), (t, at, g, i)
             assert torch.isnan(lse[0, i, 4 * g : 4 * g + 4]).all() == (sees and at >= 256)
+
+
+def test_the_largest_batch():
+    """1024 sequences of up to 64 drafts, pieces of 16 and more in a share;
+    some of them against the answer for each alone."""
+    batch, n, capacity = 1024, 64, 134
+    g = torch.Generator(DEV).manual_seed(1)
+    records = torch.randn(batch, 4, capacity, 512, generator=g, device=DEV).to(ref.E4M3).view(torch.uint8)
+    lens = torch.randint(0, capacity - 60, (batch,), generator=gen(2)).int()
+    lens[[0, 1023]] = torch.tensor([0, capacity - 3], dtype=torch.int32)
+    weights = torch.zeros(batch, 4, capacity, device=DEV)
+    cache = RecordCache(records, lens.to(DEV), weights=weights)
+    q = torch.randn(batch, n, 16, 256, generator=g, device=DEV).bfloat16()
+    tree, counts = random_tree(batch, n), torch.randint(0, n + 1, (batch,), generator=gen(3)).int()
+    out, lse = cache.tree_decode(q, tree, counts=counts.to(DEV))
+    cache.key_weights(q, lse, tree, counts=counts.to(DEV))
+    small = RecordCache.allocate(batch, 32, device=DEV)
+    cache.evict(small, 32, sink=4, local=8)
+    for b in (0, 1, 63, 64, 511, 700, 1022, 1023):
+        one = RecordCache(records[b : b + 1].clone(), [int(lens[b])], weights=torch.zeros(1, 4, capacity, device=DEV))
+        want, want_lse, want_weights, errors = answer(one, q[b : b + 1], tree[b : b + 1], counts[b : b + 1], 0.0)
+        ref.check("out", out[b : b + 1], want, errors[0])
+        ref.check("lse", lse[b : b + 1], want_lse, errors[1])
+        ref.check("weights", weights[b : b + 1], want_weights, errors[2] + want_weights * 2.0**-24)
+        length = int(lens[b])
+        for head in range(4):
+            stay = ref.kept(weights[b, head].tolist(), length, 32, 4, 8)
+            assert torch.equal(small.records[b, head, : len(stay)], records[b, head, stay])
+    assert torch.equal(small.lengths.cpu(), lens.clamp(max=32))
