@@ -740,7 +740,6 @@ struct WideBuffers {
     // bits are half the bytes (32 drafts over 131072 keys 110 us with one, 98 with
     // three, then LDS bound; in 8 bits 98 with one or two)
     constexpr int SETS = RT == 1 && F::BYTES == RECORD_FOUR ? 3 : 1;
-    constexpr int AHEAD = 2;
     std::conditional_t<V, typename F::V, typename F::K> in[SETS];
     bool hole[SETS];    // of the tile in registers
     Tile ahead;         // the next to load: its page is read a step before it is used
@@ -816,20 +815,15 @@ struct WideBuffers {
         v4f acc[RT][2];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) acc[rt][0] = acc[rt][1] = v4f{0.f, 0.f, 0.f, 0.f};
-        const uint4* kb = from + pair * 2 * IMG_TILE + ln;
-        uint4 ring[AHEAD + 1];
 #pragma unroll
-        for (int n = 0; n < AHEAD; ++n) ring[n] = kb[((n & 1) * STEPS + (n >> 1)) * WAVE];
+        for (int step = 0; step < STEPS; ++step)
 #pragma unroll
-        for (int n = 0; n < 2 * STEPS; ++n) {
-          const int to = n + AHEAD;
-          if (to < 2 * STEPS) ring[to % (AHEAD + 1)] = kb[((to & 1) * STEPS + (to >> 1)) * WAVE];
-          const v8bf kk = __builtin_bit_cast(v8bf, ring[n % (AHEAD + 1)]);
+          for (int x = 0; x < 2; ++x) {
+            const v8bf kk = __builtin_bit_cast(v8bf, from[((pair * 2 + x) * STEPS + step) * WAVE + ln]);
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt)
-            acc[rt][n & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kk, q[rt][n >> 1], acc[rt][n & 1], 0, 0, 0);
-          __builtin_amdgcn_sched_barrier(0);
-        }
+            for (int rt = 0; rt < RT; ++rt)
+              acc[rt][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kk, q[rt][step], acc[rt][x], 0, 0, 0);
+          }
         const bool bad0 = HOLES && (holes >> (16 * pair)) & 0xffu, bad1 = HOLES && (holes >> (16 * pair + 8)) & 0xffu;
         v8h pb[RT];
 #pragma unroll
@@ -841,15 +835,11 @@ struct WideBuffers {
         }
         const uint4* vb = from + KBUF + pair * 16 * WAVE + ln;
 #pragma unroll
-        for (int n = 0; n < AHEAD; ++n) ring[n] = vb[n * WAVE];
-#pragma unroll
         for (int i = 0; i < 16; ++i) {
-          if (i + AHEAD < 16) ring[(i + AHEAD) % (AHEAD + 1)] = vb[(i + AHEAD) * WAVE];
-          const v8h va = __builtin_bit_cast(v8h, ring[i % (AHEAD + 1)]);
+          const v8h va = __builtin_bit_cast(v8h, vb[i * WAVE]);
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt)
             sums.o[rt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb[rt], sums.o[rt][i], 0, 0, 0);
-          __builtin_amdgcn_sched_barrier(0);
         }
       }
       if (!V) advance(it, set);

@@ -165,12 +165,11 @@ __global__ __launch_bounds__(512) void k_attend_plan(AttendArgs a, int blocks) {
     const int once = least(AT_CUS);
     if (once + AT_COST <= 2 * (length + AT_COST)) length = once;
   }
-  const int shares = ceil_div(most, length), even = shares ? ceil_div(most, shares) : 0;
-  s_even[u] = even;
-  __syncthreads();
-  // the longest pieces first
+  // neighbours with the most pairs first
   int rank = 0;
-  for (int v = 0; v < groups; ++v) rank += s_even[v] > even || (s_even[v] == even && v < u);
+  for (int v = 0; v < groups; ++v) rank += s_pairs[v] > most || (s_pairs[v] == most && v < u);
+  const int shares = ceil_div(most, length), even = shares ? ceil_div(most, shares) : 1;
+  s_even[u] = even;
   s_by_rank[u] = 0;
   __syncthreads();
   if (u < groups) {
@@ -185,7 +184,7 @@ __global__ __launch_bounds__(512) void k_attend_plan(AttendArgs a, int blocks) {
   if (u < groups)
 #pragma unroll
     for (int r = 0; r < AT_NEAR; ++r)  // (neighbours with rows come first in a list)
-      if (r < count) part.parts[list * blocks + first + r] = Parts{s_by_rank[rank] + r, live, own[r] ? ceil_div(own[r], even) : 0};
+      if (r < count) part.parts[list * blocks + first + r] = Parts{s_by_rank[rank] + r, live, ceil_div(own[r], even)};
   // piece u is of the last neighbours that begin at or before it
   Piece piece{0, 0, 0, 0};
   if (u < s_sums[0]) {
@@ -270,7 +269,7 @@ __global__ __launch_bounds__(512) void k_attend(AttendArgs a, int blocks) {
         for (int r = 0; r < 4; ++r) scores[x][r] = (seen >> r) & 1u ? scores[x][r] : -INFINITY;
       }
     };
-    wide.template walk<F, AT_RT, PAGED, true>(a.c, b, g, tok.keys, reach, p0, p1, q, sums, a.cap,
+    wide.template walk<F, AT_RT, PAGED>(a.c, b, g, tok.keys, reach, p0, p1, q, sums, a.cap,
                                         wave * AT_RT * 16 < tok.rows, hide_rows);
     sums.total();
     const int lane = anew(threadIdx.x) & 63, kb = lane >> 4, row0 = wave * AT_RT * 16 + (lane & 15);

@@ -283,8 +283,7 @@ __global__ __launch_bounds__(512) void k_tree_wide(TreeArgs a) {
       hide<EDGE>(scores, seq, a.window, EDGE ? s_sight[(wave * RT + rt) * 16 + (ln & 15)] : Sight{0, 0},
                  EDGE ? reach.pair(pair) * TR_PAIR + 4 * (ln >> 4) : 0, bad0, bad1);
     };
-    constexpr bool RING = RT == 1 || F::BYTES == RECORD_FOUR;
-    wide.template walk<F, RT, PAGED, RING>(a.c, b, g, seq.keys, reach, p0 - first, p1 - first, q, sums, a.cap, true, hide_rows);
+    wide.template walk<F, RT, PAGED>(a.c, b, g, seq.keys, reach, p0 - first, p1 - first, q, sums, a.cap, true, hide_rows);
     sums.total();
     const Partials part = partials();
     sums.store(part, part.tile(g, k, b), wave * RT, seq.rows, lane);
