@@ -378,7 +378,8 @@ int skv_tree_decode_window(const skv_record_cache *cache, const skv_rows *q, int
 /* Attention of a chain of n tokens of every sequence, up to 2^26 in all:
  * skv_tree_decode without a tree, with window >= 1 skv_tree_decode_window
  * (window 0: none).  workspace: skv_attend_workspace(batch, n) bytes, NULL
- * where that is 0. */
+ * where that is 0.  out may be q's contiguous rows in place; out and lse of
+ * more than 64 tokens share no other memory with q. */
 int skv_attend(const skv_record_cache *cache, const skv_rows *q, int n, const int32_t *counts, float cap,
                int window, int sink, void *out, float *lse, void *workspace, int64_t workspace_bytes,
                void *stream);

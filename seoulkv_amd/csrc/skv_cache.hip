@@ -486,6 +486,13 @@ int skv_attend(const skv_record_cache* cache, const skv_rows* q, int n, const in
   const uint64_t rows = (uint64_t)cache->batch * n * QHEADS;
   c.memory("out", out, rows * SKV_DIM * 2, 16);
   if (c.ok()) c.memory("lse", lse, rows * 4, 4);
+  if (c.ok() && n > TREE_MAX_DRAFTS) {
+    // some blocks write results while others read queries (fewer tokens are read by
+    // one kernel and written by the next)
+    const int64_t st = QHEADS * SKV_DIM;
+    in_place_or_apart(c, "out", a.q, Rows{out, n * st, st, SKV_DIM}, batch, n, QHEADS, SKV_DIM, 2);
+    c.require(!overlap(lse, rows * 4, a.q.data, 2 * extent(a.q, batch, n, QHEADS, SKV_DIM)), "lse overlaps q");
+  }
   if (c.ok()) workspace_of(c, workspace, workspace_bytes, skv_attend_workspace(batch, n));
   if (!c.ok()) return c.code;
   a.n = n;

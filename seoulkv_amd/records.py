@@ -369,7 +369,9 @@ class RecordCache:
         sequence, any number, that lie in the slots behind the committed ones
         (``write`` put them there) and of which each sees what :meth:`tree_decode`
         lets a chain see, the committed slots and the tokens up to itself.
-        Arguments and results are those of ``tree_decode``."""
+        Arguments and results are those of ``tree_decode``.  ``out`` may be a
+        contiguous ``q``; otherwise ``out`` and ``lse`` of more than 64 tokens
+        share no memory with ``q``."""
         desc = self._open()
         q = self._queries(q, self.capacity)
         n = q.shape[1]
