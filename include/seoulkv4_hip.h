@@ -499,6 +499,8 @@ const char *skv_last_error(void *handle);
 
 /* Library build identification. */
 const char *skv_version(void);
+/* A hash of the sources that the library was built from, "" if its build gave none. */
+const char *skv_sources(void);
 
 #ifdef __cplusplus
 }

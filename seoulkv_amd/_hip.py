@@ -131,8 +131,23 @@ def load_library() -> ctypes.CDLL:
             f"SeoulKV4 HIP library missing at {LIB_PATH}; build it with "
             "`python -m seoulkv_amd.build` (gfx950)"
         )
-    _lib = _bind(ctypes.CDLL(str(LIB_PATH)))
+    _lib = _bind(_of_these_sources(ctypes.CDLL(str(LIB_PATH)), LIB_PATH))
     return _lib
+
+
+def _of_these_sources(lib: ctypes.CDLL, path: Path) -> ctypes.CDLL:
+    """``lib``, unless it was built from other sources than lie beside it
+    (without sources there is nothing to compare)."""
+    from seoulkv_amd import build  # (not at import: it is run as a program too)
+
+    if build.CSRC.is_dir() and build.HEADER.exists():
+        built = getattr(lib, "skv_sources", None)
+        if built is not None:
+            built.restype = ctypes.c_char_p
+        if built is None or built().decode() != build.sources_id():
+            raise RuntimeError(f"{path} was built from other sources than {build.CSRC} holds; build it again "
+                               "(`__graft_entry__.build()`, or `python -m seoulkv_amd.build`)")
+    return lib
 
 
 def load_trace_library() -> ctypes.CDLL | None:
@@ -142,7 +157,7 @@ def load_trace_library() -> ctypes.CDLL | None:
     device timestamps, read with :meth:`Runtime.trace_blocks`."""
     global _trace_lib
     if _trace_lib is None and TRACE_LIB_PATH.exists():
-        lib = _bind(ctypes.CDLL(str(TRACE_LIB_PATH)))
+        lib = _bind(_of_these_sources(ctypes.CDLL(str(TRACE_LIB_PATH)), TRACE_LIB_PATH))
         lib.skv_trace_blocks.restype = ctypes.c_int32
         lib.skv_trace_blocks.argtypes = [ctypes.c_void_p]
         _trace_lib = lib
@@ -203,6 +218,7 @@ def _bind(lib: ctypes.CDLL) -> ctypes.CDLL:
         "skv_destroy": (None, [vp]),
         "skv_last_error": (ctypes.c_char_p, [vp]),
         "skv_version": (ctypes.c_char_p, []),
+        "skv_sources": (ctypes.c_char_p, []),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)

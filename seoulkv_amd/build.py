@@ -7,6 +7,7 @@ the package; ``seoulkv_amd._hip`` loads it from this directory.
 
 from __future__ import annotations
 
+import hashlib
 import os
 import shutil
 import subprocess
@@ -17,6 +18,7 @@ from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
+HEADER = HERE.parent / "include" / "seoulkv4_hip.h"
 LIB = HERE / "libseoulkv4_hip.so"
 SOURCES = ["skv_runtime.hip", "skv_kernels.hip", "skv_dense.hip", "skv_cache.hip",
            "skv_rotary.hip", "skv_norm.hip", "skv_tree.hip", "skv_attend.hip", "skv_evict.hip"]
@@ -59,6 +61,16 @@ SANITIZE_FLAGS = [
 ]
 
 
+def sources_id() -> str:
+    """What ``skv_sources()`` of a library built from this tree says: a hash of
+    the sources, the header and the flags (but for the architecture)."""
+    digest = hashlib.sha256(" ".join(f for f in FLAGS if not f.startswith("--offload-arch")).encode())
+    for path in [*sorted(CSRC.iterdir()), HEADER]:
+        if path.suffix in (".hip", ".h"):
+            digest.update(path.name.encode() + b"\0" + path.read_bytes())
+    return digest.hexdigest()[:32]
+
+
 def _run(cmd: list[str], verbose: bool) -> None:
     if verbose:
         print(" ".join(cmd), flush=True)
@@ -79,13 +91,17 @@ def build(verbose: bool = False, trace: bool = False, sanitize_dir: Path | None 
     builds ``libseoulkv4_hip_asan.so`` there, its host code instrumented with
     the address and undefined-behaviour sanitizers (tests only: a program
     that loads it must itself be linked with ``-fsanitize=address,undefined``
-    by clang, which provides the runtime)."""
+    by clang, which provides the runtime).  A library that is there goes first:
+    a build that fails leaves none."""
     if sanitize_dir is not None:
         lib = Path(sanitize_dir) / "libseoulkv4_hip_asan.so"
     else:
         lib = LIB.with_name("libseoulkv4_hip_trace.so") if trace else LIB
     tmp = lib.with_suffix(".so.tmp")
-    extra = ["-DSKV_TRACE"] if trace else []
+    lib.unlink(missing_ok=True)
+    extra = [f'-DSKV_SOURCES="{sources_id()}"']
+    if trace:
+        extra.append("-DSKV_TRACE")
     if sanitize_dir is not None:
         extra += SANITIZE_FLAGS
     with tempfile.TemporaryDirectory() as objects:

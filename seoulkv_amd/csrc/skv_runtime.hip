@@ -348,6 +348,11 @@ extern "C" {
 
 const char* skv_version(void) { return "seoulkv4-hip gfx950 1"; }
 
+#ifndef SKV_SOURCES
+#define SKV_SOURCES ""
+#endif
+const char* skv_sources(void) { return SKV_SOURCES; }
+
 const char* skv_last_error(void* handle) {
   if (!handle) return g_create_error.c_str();
   return static_cast<Handle*>(handle)->error.c_str();
