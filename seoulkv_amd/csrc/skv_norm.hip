@@ -539,16 +539,19 @@ int split_heads(int64_t blocks, int heads, int batch, int target, int& per) {
 
 constexpr int NG_BLOCKS = 1024;  // blocks of the gradient: 4 of 4 waves on each of 256 CUs
 
-// Blocks of the gradient along tokens (x) and heads (y); `per` heads each.
+// Blocks of the gradient along tokens (x) and heads (y); `per` heads each, with
+// one weight for all of them a multiple of the `batch` in flight (half of it, the
+// other half loaded twice, in rows of 100 BF16 elements: 1000 tokens x 8 heads 15.7
+// us, 11.4 so; 256 x 20 11.9 and 10.0; 1 x 20 6.2 and 7.0, less than the host's call).
 struct GradGrid {
   int x, y, per;
-  GradGrid(int64_t tokens, int heads, const Shape& s, bool per_head) {
-    const int64_t groups = (tokens * s.lanes + RO_BLOCK - 1) / RO_BLOCK;
+  GradGrid(int64_t tokens, int heads, int lanes, int batch, bool per_head) {
+    const int64_t groups = (tokens * lanes + RO_BLOCK - 1) / RO_BLOCK;
     if (per_head) {
       per = 1;
       y = heads;
     } else {
-      y = split_heads(groups, heads, s.by8 && s.lanes < 64 ? 4 : 2, NG_BLOCKS, per);
+      y = split_heads(groups, heads, batch, NG_BLOCKS, per);
     }
     const int64_t most = NG_BLOCKS / y > 0 ? NG_BLOCKS / y : 1;
     x = (int)(groups < most ? groups : most);
@@ -568,18 +571,22 @@ void norm_typed(const NormRows& a, const Rows& y, hipStream_t st) {
   });
 }
 
+// Returns the partial rows of dw.
 template <typename T>
-void grad_typed(const NormRows& a, const Rows& g, const Rows& y, float* partial, hipStream_t st) {
+int grad_typed(const NormRows& a, const Rows& g, const Rows& y, float* partial, hipStream_t st) {
   const Shape s(rows_by_8(a.x, sizeof(T)) && rows_by_8(g, sizeof(T)) && rows_by_8(y, sizeof(T)) &&
                     weight_by_8(a.w, sizeof(T)),
                 a.r.pairs, a.dim);
   const int64_t tokens = (int64_t)a.batch * a.n;
-  const GradGrid grid(tokens, a.heads, s, a.w.sh != 0);
+  int rows = 0;
   with_shape(s, [&](auto n, auto l, auto per_lane) {
+    const GradGrid grid(tokens, a.heads, l(), batch_of<n(), per_lane()>, a.w.sh != 0);
+    rows = grid.x * grid.y;
     auto kernel = a.w.sh ? k_norm_grad<T, n(), l(), per_lane(), true> : k_norm_grad<T, n(), l(), per_lane(), false>;
     hipLaunchKernelGGL(kernel, dim3(grid.x, grid.y), dim3(RO_BLOCK), 0, st, a.r, a.w, g, a.x, y, tokens, s.units, a.n,
                        a.heads, a.dim, grid.per, a.interleaved, partial);
   });
+  return rows;
 }
 
 }  // namespace
@@ -600,14 +607,9 @@ size_t norm_grad_workspace(int64_t tokens, int heads, int dim, bool per_head) {
 void launch_norm_grad(const NormRows& a, const Rows& g, const Rows& y, int dtype, void* dw, int dw_dtype,
                       float* partial, hipStream_t st) {
   auto run = dtype == 0 ? grad_typed<BF16> : dtype == 1 ? grad_typed<FP16> : grad_typed<float>;
-  run(a, g, y, partial, st);
-  const int size = dtype == 2 ? 4 : 2;
-  const Shape s(rows_by_8(a.x, size) && rows_by_8(g, size) && rows_by_8(y, size) && weight_by_8(a.w, size), a.r.pairs,
-                a.dim);
-  const GradGrid grid((int64_t)a.batch * a.n, a.heads, s, a.w.sh != 0);
-  const int rows = a.w.sh ? a.heads : 1;
-  hipLaunchKernelGGL(k_norm_weight, dim3((a.dim + 63) / 64, rows), dim3(1024), 0, st, partial,
-                     grid.x * grid.y / rows, a.dim, dw, dw_dtype);
+  const int shares = run(a, g, y, partial, st), rows = a.w.sh ? a.heads : 1;
+  hipLaunchKernelGGL(k_norm_weight, dim3((a.dim + 63) / 64, rows), dim3(1024), 0, st, partial, shares / rows, a.dim, dw,
+                     dw_dtype);
 }
 
 void launch_cache_write_normed(const WriteArgs& a, const NormArgs& qw, const NormArgs& kw, hipStream_t st) {
