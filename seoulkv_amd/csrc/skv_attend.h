@@ -50,6 +50,7 @@ struct Sequence {
 // come in slot order; with one the pairs between the sink's and the window's
 // are left out.
 struct Reach {
+  static constexpr bool ENDS = true;  // see WideBuffers
   int whole, all;       // numbers of pairs
   int sink, sink_pairs; // whole ones in the sink; pairs of the sink
   int late, window;     // first whole pair of every window; first pair of some window
@@ -80,6 +81,14 @@ struct Reach {
     i -= sink_pairs - sink;
     return i < late - window ? window + i : open + i - (late - window);
   }
+};
+
+// The same without a window: the pairs in slot order.
+struct AllPairs {
+  static constexpr bool ENDS = false;
+  int whole, all;
+  __device__ AllPairs(const Sequence& s, const Window&) : whole(s.len / TR_PAIR), all((s.keys + TR_PAIR - 1) / TR_PAIR) {}
+  __device__ __forceinline__ int pair(int i) const { return i; }
 };
 
 // Pairs of a sequence; with WHOLE one without rows counts too.
@@ -624,7 +633,13 @@ struct RowSums {
   }
 };
 
-// Which of slots t .. t + 3 a row sees (bits 0 .. 3).
+// Which of slots t .. t + 3 a row sees (bits 0 .. 3): of the drafts those in `bits`;
+// with a window.
+__device__ __forceinline__ uint32_t seen4(const Sequence& s, const Window&, uint64_t bits, int t) {
+  const int j = t - s.len;
+  if (j < 0) return (uint32_t)((bits << min(-j, 63)) | ((1ull << min(-j, 63)) - 1ull));
+  return j < 64 ? (uint32_t)(bits >> j) : 0u;
+}
 __device__ __forceinline__ uint32_t seen4(const Sequence& s, const Window& w, const Sight& r, int t) {
   const int j = t - s.len;
   uint64_t drafts = r.bits;
@@ -637,8 +652,8 @@ __device__ __forceinline__ uint32_t seen4(const Sequence& s, const Window& w, co
 
 // The scores of invisible keys of a pair become -inf: of tiles without a page,
 // and with EDGE of those that the row does not see.  t: the lane's first key.
-template <bool EDGE>
-__device__ __forceinline__ void hide(v4f (&s)[2], const Sequence& seq, const Window& w, const Sight& row, int t,
+template <bool EDGE, typename Row>
+__device__ __forceinline__ void hide(v4f (&s)[2], const Sequence& seq, const Window& w, const Row& row, int t,
                                      bool bad0, bool bad1) {
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
@@ -679,6 +694,12 @@ __device__ __forceinline__ int anew(int x) {
 // twice buffered, and every wave reads its operands there; the queries stay in
 // registers.  (So what is not needed in the walk is formed anew after it: a spill of
 // loaded records would wait for them.)
+//
+// Pairs without ENDS, a tree's without a window, are walked with less beside the
+// operands: pages are read with their tiles, holes tested in every step.  With the
+// window's form scalar registers ran out and operands were read from LDS one by one
+// (paged, 32 drafts over 131072 keys 120 us, 103 so; of 24 ragged sequences 99 and 87;
+// 64 capped drafts, contiguous, 221 and 214).
 struct WideBuffers {
   static constexpr int KBUF = 2 * 2 * IMG_TILE;   // uint4: [pair][tile][step][lane]
   static constexpr int VBUF = 2 * 16 * WAVE;      // uint4: [pair][dim of 16][lane], tile x in half x
@@ -690,11 +711,11 @@ struct WideBuffers {
   // Adds pairs p0 .. p1 - 1 of `reach` to the sums of the wave's rows; waves
   // that are not `active` only load.  hide_rows(edge, rt, scores, pair, lane,
   // bad0, bad1) hides what a row does not see.
-  template <typename F, int RT, bool PAGED, typename Hide>
-  __device__ __forceinline__ void walk(const CacheView& c, int b, int g, int keys, const Reach& reach, int p0, int p1,
+  template <typename F, int RT, bool PAGED, typename Pairs, typename Hide>
+  __device__ __forceinline__ void walk(const CacheView& c, int b, int g, int keys, const Pairs& reach, int p0, int p1,
                                        const v8bf (&q)[RT][STEPS], RowSums<RT>& sums, float cap, bool active,
                                        Hide hide_rows) {
-    if constexpr (PAGED) {
+    if constexpr (PAGED && Pairs::ENDS) {
       // (pages that are none are rare: looked for once and not in every step,
       // whose wait for the flags took a sixth of the time)
       int hole = 0;
@@ -707,7 +728,7 @@ struct WideBuffers {
         return;
       }
     }
-    forms<F, RT, PAGED, false>(c, b, g, keys, reach, p0, p1, q, sums, cap, active, hide_rows);
+    forms<F, RT, PAGED, PAGED && !Pairs::ENDS>(c, b, g, keys, reach, p0, p1, q, sums, cap, active, hide_rows);
   }
 
  private:
@@ -715,8 +736,8 @@ struct WideBuffers {
   // that do V (each SIMD has one of both): registers that two branches load are
   // copied where the branches meet, which waits for the loads.  Both take the
   // same barriers.
-  template <typename F, int RT, bool PAGED, bool HOLES, typename Hide>
-  __device__ __forceinline__ void forms(const CacheView& c, int b, int g, int keys, const Reach& reach, int p0, int p1,
+  template <typename F, int RT, bool PAGED, bool HOLES, typename Pairs, typename Hide>
+  __device__ __forceinline__ void forms(const CacheView& c, int b, int g, int keys, const Pairs& reach, int p0, int p1,
                                         const v8bf (&q)[RT][STEPS], RowSums<RT>& sums, float cap, bool active,
                                         Hide hide_rows) {
     if (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) >= 4) {
@@ -727,8 +748,8 @@ struct WideBuffers {
     }
   }
 
-  template <typename F, int RT, bool PAGED, bool HOLES, bool V, typename Hide>
-  __device__ __forceinline__ void form(const CacheView& c, int b, int g, int keys, const Reach& reach, int p0, int p1,
+  template <typename F, int RT, bool PAGED, bool HOLES, bool V, typename Pairs, typename Hide>
+  __device__ __forceinline__ void form(const CacheView& c, int b, int g, int keys, const Pairs& reach, int p0, int p1,
                                        const v8bf (&q)[RT][STEPS], RowSums<RT>& sums, float cap_at, bool active,
                                        Hide hide_rows) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -742,17 +763,18 @@ struct WideBuffers {
     constexpr int SETS = RT == 1 && F::BYTES == RECORD_FOUR ? 3 : 1;
     std::conditional_t<V, typename F::V, typename F::K> in[SETS];
     bool hole[SETS];    // of the tile in registers
-    Tile ahead;         // the next to load: its page is read a step before it is used
+    Tile ahead;         // the next to load: with ENDS its page is read a step before it is used
     auto find = [&](int it) {  // (past the last pair: its last tile again, not used)
       const int pair = min(p0 + 2 * it + sp, p1 - 1);
       ahead = tile_at<F::BYTES, PAGED>(c, b, g, reach.pair(pair) * TR_PAIR + 16 * sx, keys);
     };
     // (set: it % SETS, known to the compiler)
     auto load = [&](int it, int set) {
+      if constexpr (!Pairs::ENDS) find(it);
       if constexpr (V) F::template load_v<false, true>(in[set], ahead, anew(lane));
       else F::template load_k<false>(in[set], ahead, anew(lane));
       hole[set] = ahead.bad;
-      find(it + 1);
+      if constexpr (Pairs::ENDS) find(it + 1);
     };
     auto widen = [&](int it, int set) {
       uint4* to = buf + (it & 1) * BUF;
@@ -784,7 +806,7 @@ struct WideBuffers {
       if (SETS > 1 || it + 1 < steps) widen(it + 1, set);
       if (SETS > 1 || it + 2 < steps) load(it + 1 + SETS, set);
     };
-    find(0);
+    if constexpr (Pairs::ENDS) find(0);
 #pragma unroll
     for (int d = 0; d < SETS; ++d) load(d, d);
     widen(0, 0);

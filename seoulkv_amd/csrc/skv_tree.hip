@@ -252,11 +252,12 @@ __global__ __launch_bounds__(RW * KW * 64) void k_tree(TreeArgs a) {
 
 // More than 16 drafts: 8 row waves of 16 RT rows would each widen the same
 // records.  Here they widen them together (WideBuffers).
-template <typename F, int RT, bool PAGED>
+template <typename F, int RT, bool PAGED, bool WINDOW>
 __global__ __launch_bounds__(512) void k_tree_wide(TreeArgs a) {
   constexpr int TILES = RT * 8;
+  typedef std::conditional_t<WINDOW, Sight, uint64_t> Row;  // (the drafts alone)
   __shared__ WideBuffers wide;
-  __shared__ Sight s_sight[TILES * 16];
+  __shared__ Row s_sight[TILES * 16];
   __shared__ int s_start[CACHE_MAX_BATCH + 1];
   const int g = blockIdx.y, k = blockIdx.x;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -269,9 +270,12 @@ __global__ __launch_bounds__(512) void k_tree_wide(TreeArgs a) {
   };
   each_piece(a, s_start, [&](int b, int first, int p0, int p1) {
     const Sequence seq = Sequence(a.c, a.counts, a.n, b).uniform();
-    const Reach reach(seq, a.window);
-    for (int r = threadIdx.x; r < TILES * 16; r += 512)
-      s_sight[r] = r < seq.rows ? sight_of(seq, a.window, row_mask(a.tree, a.n, b, r / H)) : Sight{0, 0};
+    const std::conditional_t<WINDOW, Reach, AllPairs> reach(seq, a.window);
+    for (int r = threadIdx.x; r < TILES * 16; r += 512) {
+      const uint64_t bits = r < seq.rows ? row_mask(a.tree, a.n, b, r / H) : 0;
+      if constexpr (WINDOW) s_sight[r] = sight_of(seq, a.window, bits);
+      else s_sight[r] = bits & seq.there();
+    }
     if (threadIdx.x == 0) wide.nan = 0;
     v8bf q[RT][STEPS];
     load_queries<F>(q, a.q, b, g, 0, seq.rows, wave * RT * 16 + col, kb);
@@ -280,7 +284,7 @@ __global__ __launch_bounds__(512) void k_tree_wide(TreeArgs a) {
     sums.clear();
     auto hide_rows = [&](auto edge, int rt, v4f (&scores)[2], int pair, int ln, bool bad0, bool bad1) {
       constexpr bool EDGE = decltype(edge)::value;
-      hide<EDGE>(scores, seq, a.window, EDGE ? s_sight[(wave * RT + rt) * 16 + (ln & 15)] : Sight{0, 0},
+      hide<EDGE>(scores, seq, a.window, EDGE ? s_sight[(wave * RT + rt) * 16 + (ln & 15)] : Row{},
                  EDGE ? reach.pair(pair) * TR_PAIR + 4 * (ln >> 4) : 0, bad0, bad1);
     };
     wide.template walk<F, RT, PAGED>(a.c, b, g, seq.keys, reach, p0 - first, p1 - first, q, sums, a.cap, true, hide_rows);
@@ -570,8 +574,11 @@ void tree_rows(const TreeArgs& a, hipStream_t st) {
   // itself; 64 drafts 154 us, 219 by 8)
   else if (tiles <= 2) hipLaunchKernelGGL((k_tree<F, 2, 1, 8, PAGED>), grid, dim3(512), 0, st, a);
   else if (tiles <= 4) hipLaunchKernelGGL((k_tree<F, 2, 2, 4, PAGED>), grid, dim3(512), 0, st, a);
-  else if (tiles <= 8) hipLaunchKernelGGL((k_tree_wide<F, 1, PAGED>), grid, dim3(512), 0, st, a);
-  else hipLaunchKernelGGL((k_tree_wide<F, 2, PAGED>), grid, dim3(512), 0, st, a);
+  else {
+    auto wide = tiles <= 8 ? (a.window.size ? k_tree_wide<F, 1, PAGED, true> : k_tree_wide<F, 1, PAGED, false>)
+                           : (a.window.size ? k_tree_wide<F, 2, PAGED, true> : k_tree_wide<F, 2, PAGED, false>);
+    hipLaunchKernelGGL(wide, grid, dim3(512), 0, st, a);
+  }
 }
 
 template <typename F, bool PAGED, bool WINDOW>
