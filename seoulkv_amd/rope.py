@@ -148,20 +148,20 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, table: RotaryTable, *,
     transposed map: given the gradient with respect to the result it returns
     the gradient with respect to ``x`` (and, for scale 1, undoes the turn).
     Enqueued on PyTorch's current stream; FP32 arithmetic, rounded once."""
-    dtype = _checked_rows(x, positions, table)
+    shape, dtype = _checked_rows(x, positions, table)
     _no_grad("rotary", x, out)
-    given, out = out, _output_like(x, out)
+    given, out = out, _output_like(x, shape, out)
     if x.numel() == 0:
         return out
     positions = positions.contiguous()
     _hip.call_on(x.device.index, "skv_rotary", table._desc, _hip.rows_desc(x), _hip.rows_desc(out),
-                 dtype, *_sizes(x, positions), bool(transpose))
+                 dtype, *_sizes(shape, positions), bool(transpose))
     _written(given)
     return out
 
 
-def _checked_rows(x, positions, table) -> int:
-    """The C type of rows that are turned."""
+def _checked_rows(x, positions, table) -> tuple[torch.Size, int]:
+    """The shape and C type of rows that are turned."""
     if not isinstance(table, RotaryTable):
         raise TypeError("table must be a RotaryTable")
     shape, dtype = x.shape, _DTYPES.get(x.dtype)
@@ -173,25 +173,23 @@ def _checked_rows(x, positions, table) -> int:
         raise ValueError("expected int32 or int64 positions [n] or [batch, n]")
     if not x.device == positions.device == table.device:
         raise ValueError("x, positions and table must be on one device")
-    return dtype
+    return shape, dtype
 
 
-def _output_like(x, out):
+def _output_like(x, shape, out):
     if out is None:
-        out = x.new_empty(x.shape)
-    elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
+        out = x.new_empty(shape)
+    elif out.shape != shape or out.dtype != x.dtype or out.device != x.device:
         raise ValueError("out must have x's shape, type and device")
-    if x.numel() and (x.stride(-1) != 1 or out.stride(-1) != 1):
+    if (x.stride(-1) != 1 or out.stride(-1) != 1) and x.numel():
         raise ValueError("the last dimension of x and out must be contiguous")
     return out
 
 
-def _sizes(x, positions):
+def _sizes(shape, positions):
     """Sizes and positions (contiguous) of rows as the C entry points take them."""
-    batch = x.shape[0] if x.dim() == 4 else 1
-    per_batch = x.shape[-3] if positions.dim() == 2 else 0
-    return (batch, x.shape[-3], x.shape[-2], x.shape[-1], positions.data_ptr(), per_batch,
-            positions.dtype == torch.int64)
+    batch, (n, heads, dim) = shape[0] if len(shape) == 4 else 1, shape[-3:]
+    return batch, n, heads, dim, positions.data_ptr(), n if positions.dim() == 2 else 0, positions.dtype == torch.int64
 
 
 def _head_norm(name, weight, eps, dtype, heads, dim, device) -> tuple[_hip.HeadNorm, torch.Tensor]:
@@ -214,15 +212,15 @@ def norm_rotary(x: torch.Tensor, positions: torch.Tensor, table: RotaryTable, we
     and key heads of a fused projection), of ``x``'s type or FP32; the other
     arguments are :func:`rotary`'s.  FP32 arithmetic, rounded once; squares are
     summed in FP32, so a head whose sum of squares passes its range gives 0."""
-    dtype = _checked_rows(x, positions, table)
-    norm, weight = _head_norm("weight", weight, eps, x.dtype, *x.shape[-2:], x.device)
+    shape, dtype = _checked_rows(x, positions, table)
+    norm, weight = _head_norm("weight", weight, eps, x.dtype, *shape[-2:], x.device)
     _no_grad("norm_rotary", x, weight, out)
-    given, out = out, _output_like(x, out)
+    given, out = out, _output_like(x, shape, out)
     if x.numel() == 0:
         return out
     positions = positions.contiguous()
     _hip.call_on(x.device.index, "skv_norm_rotary", table._desc, norm, _hip.rows_desc(x), _hip.rows_desc(out),
-                 dtype, *_sizes(x, positions))
+                 dtype, *_sizes(shape, positions))
     _written(given)
     return out
 
@@ -235,20 +233,20 @@ def norm_rotary_grad(grad: torch.Tensor, x: torch.Tensor, positions: torch.Tenso
     result (``x``'s shape and type, its last dimension contiguous).  ``out``: a
     tensor like ``x`` for the first, which may be ``grad`` or ``x`` itself.  The
     weight's is summed in FP32 in a fixed order, the same bits every time."""
-    dtype = _checked_rows(x, positions, table)
-    if grad.shape != x.shape or grad.dtype != x.dtype or grad.device != x.device:
+    shape, dtype = _checked_rows(x, positions, table)
+    if grad.shape != shape or grad.dtype != x.dtype or grad.device != x.device:
         raise ValueError("grad must have x's shape, type and device")
-    norm, weight = _head_norm("weight", weight, eps, x.dtype, *x.shape[-2:], x.device)
+    norm, weight = _head_norm("weight", weight, eps, x.dtype, *shape[-2:], x.device)
     _no_grad("norm_rotary_grad", grad, x, weight, out)
-    given, out = out, _output_like(x, out)
+    given, out = out, _output_like(x, shape, out)
     if x.numel() == 0:
         return out, torch.zeros_like(weight)
     if grad.stride(-1) != 1:
         grad = grad.contiguous()
     dweight = torch.empty_like(weight)
     positions = positions.contiguous()
-    sizes = _sizes(x, positions)
-    size = _hip.load_library().skv_norm_grad_workspace(sizes[0] * sizes[1], *x.shape[-2:], weight.dim() == 2)
+    sizes = _sizes(shape, positions)
+    size = _hip.load_library().skv_norm_grad_workspace(sizes[0] * sizes[1], *shape[-2:], weight.dim() == 2)
     work = torch.empty(size, dtype=torch.uint8, device=x.device)
     _hip.call_on(x.device.index, "skv_norm_rotary_grad", table._desc, norm, _hip.rows_desc(grad), _hip.rows_desc(x),
                  _hip.rows_desc(out), dtype, *sizes, dweight.data_ptr(), work.data_ptr(), size)
