@@ -457,12 +457,15 @@ __global__ __launch_bounds__(weight_waves(TILES) * 64, 4) void k_key_weights(Wei
   const Window window = WINDOW ? a.window : Window{0, 0};
   const int total = a.c.batch == 1 ? sequence_pairs<true>(Sequence(a.c, a.counts, a.n, 0).uniform(), window)
                                    : sequence_starts<true>(a.c, a.counts, a.n, window, s_start);
-  if (WINDOW && !a.accumulate) {  // the pairs that no row sees
-    for (int b = 0; b < a.c.batch; ++b) {
-      const Sequence seq(a.c, a.counts, a.n, b);
-      const Reach reach(seq, window);
-      for (int t = reach.sink_pairs * TR_PAIR + k * WAVES * 64 + threadIdx.x; t < reach.window * TR_PAIR;
-           t += gridDim.x * WAVES * 64)
+  if (WINDOW && !a.accumulate) {
+    // the pairs that no row sees: several blocks a sequence, or several sequences a
+    // block (every block at all of them, 1024 sequences of 400 slots 568 us, 61 so)
+    const int parts = max((int)gridDim.x / a.c.batch, 1);
+    for (int u = k; u < a.c.batch * parts; u += gridDim.x) {
+      const int b = u / parts, part = u % parts;
+      const Reach reach(Sequence(a.c, a.counts, a.n, b), window);
+      for (int t = reach.sink_pairs * TR_PAIR + part * WAVES * 64 + threadIdx.x; t < reach.window * TR_PAIR;
+           t += parts * WAVES * 64)
         a.weights[a.c.row(b, g, t)] = 0.f;
     }
   }
