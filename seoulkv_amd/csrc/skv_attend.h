@@ -759,7 +759,8 @@ struct WideBuffers {
     const bool cap = cap_at > 0.f;
     // Tiles in flight: with one tile of rows registers are left for more, and 4
     // bits are half the bytes (32 drafts over 131072 keys 110 us with one, 98 with
-    // three, then LDS bound; in 8 bits 98 with one or two)
+    // three when that was chosen, then LDS bound, 87 now; in 8 bits 98 with one or
+    // two, 91 now)
     constexpr int SETS = RT == 1 && F::BYTES == RECORD_FOUR ? 3 : 1;
     std::conditional_t<V, typename F::V, typename F::K> in[SETS];
     bool hole[SETS];    // of the tile in registers

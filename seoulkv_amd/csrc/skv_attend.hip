@@ -20,9 +20,9 @@
 //
 // Bounds: a pair of tiles takes 256 KB of LDS reads (2048 cycles) beside as many
 // cycles of matrix cores and four fifths of that of vector units, which two waves
-// a SIMD overlap in part.  Whole calls: prompt of 16384 all visible 1890 us, 1163
-// TFLOP/s (a library product of 16384^3: 1364), 4-bit records 1830, 1202; in a window
-// of 4096 with 128 sinks 966, 1023; 2000 capped tokens of 4 bits in a window of
+// a SIMD overlap in part.  Whole calls: prompt of 16384 all visible 1900 us, 1157
+// TFLOP/s (a library product of 16384^3: 1364), 4-bit records 1845, 1192; in a window
+// of 4096 with 128 sinks 970, 1019; 2000 capped tokens of 4 bits in a window of
 // 8192 317, 855; ragged paged pieces of 6 prompts 452, 800.
 #include "skv_attend.h"
 
@@ -37,7 +37,7 @@ constexpr int AT_TOKENS = 64, AT_ROWS = AT_TOKENS * H, AT_RT = 2, AT_TILES = AT_
 constexpr int AT_FEW = 384;
 constexpr int AT_CUS = 256, AT_PIECES = 2 * AT_CUS;
 constexpr int AT_NEAR = 4;      // neighbours that are cut alike
-constexpr int AT_LEAST = 4;     // pairs of a piece (512 fresh tokens 37 us, 47 with 16)
+constexpr int AT_LEAST = 4;     // pairs of a piece (512 fresh tokens 35 to 37 us, 47 with 16)
 constexpr int AT_COST = 12;     // pairs that a piece costs beside its own: some 25 us of 2 a pair
 
 // What row `token` of a chain sees: slots [first, last] and the sink.

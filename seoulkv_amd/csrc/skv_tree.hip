@@ -20,16 +20,17 @@
 //
 // Bounds (131072 keys, contiguous, whole calls on one cache over and over): one
 // to 4 drafts 49 us (51 where several caches take turns), of which the kernel
-// 44, 6.0 TB/s, the record stream; 8 drafts 54, 16 66 (73 in turns): the wait for
+// 44, 6.0 TB/s, the record stream; 8 drafts 55, 16 66 (71 in turns): the wait for
 // records, since 256 registers a wave leave 8 waves a CU and one pair ahead; 32
-// drafts 93, 64 drafts 154, with a cap 174: multiplying and weighing, which two
+// drafts 89, 64 drafts 151, with a cap 173: multiplying and weighing, which two
 // waves a SIMD overlap little (loads two or three steps ahead changed nothing
 // there).  One draft of many ragged paged sequences: 64 of up to 8192 keys
 // (279530 in all) 113 us, 5.1 TB/s, 256 of up to 4096 (504279) 195 us, 5.3 TB/s:
 // a share holds pieces of several sequences, each with queries to stage and a
 // partial to store.  Loads pay where no wait stands between their issue and
-// their use: see the loops' notes on branches and spills (up to 19 registers of
-// the two-tile instances are spilled, outside those loops).
+// their use: see the loops' notes on branches and spills (of the two-tile instances
+// 4 to 9 registers, outside those loops; of the wide ones with a window 8 to 19, those
+// over pages partly inside).
 //
 // With a window the pairs that no row sees are left out (Reach) and the others
 // come whole ones first, so the loop over them is the same: a token of 32 ragged
@@ -37,8 +38,8 @@
 // TB/s, pieces of several sequences in a share.
 //
 // Records of 4 bits (Four) are widened with their scales by the converter.  One
-// token over 131072 keys 36 to 38 us (8 bits 51), 8 drafts 47 (56), 16 drafts 63
-// (75): 4.6 TB/s at most, since a pair takes as many vector instructions as one of
+// token over 131072 keys 35 to 38 us (8 bits 51), 8 drafts 43 (55), 16 drafts 58
+// (71): 4.6 TB/s at most, since a pair takes as many vector instructions as one of
 // 8 bits and half the bytes are in flight (two pairs ahead spilled: 41 us); from
 // 17 drafts on as 8 bits, LDS bound.  Two key halves of 4 row waves that widen
 // together: 16 drafts 76 us, 12 drafts of ragged sequences 132 against 101.
@@ -435,10 +436,12 @@ __global__ __launch_bounds__(SLICES == 1 ? 256 : SLICES * 64) void k_tree_merge(
 // over the rows in registers and then over the 16 lanes of a row group: no
 // atomics, the same bits every time.  Bound by matrix cores, vector units and
 // LDS about alike for many rows, so 4 waves on a SIMD do more than records
-// loaded ahead (32 rows over 131072 keys: 46 us, 70 with 2 waves and a pair
-// ahead; 64 rows 67); by the K halves, 256 bytes of every 512, for few (one row
-// 28 us a call, 4.8 TB/s).  4 waves leave 128 registers: 8 are spilled, outside
-// the loop over row tiles.
+// loaded ahead (32 rows over 131072 keys: 45 us, 70 with 2 waves and a pair
+// ahead; 64 rows 70); by the K halves, 256 bytes of every 512, for few (one row
+// 28 us a call, 4.8 TB/s).  4 bits as long, bound by their widening (28, 45, 70).  In
+// a window of 4096 10, 18 and 26 us, of 100000 27, 44 and 65.  4 waves leave 128
+// registers: 8 to 10 are spilled, outside the loop over row tiles, 18 to 23 with a
+// window.
 // (the 128 KB image of 64 drafts leaves room for one block, of 16 waves then)
 constexpr int weight_waves(int tiles) { return tiles > 8 ? 16 : 8; }
 
@@ -573,7 +576,7 @@ void tree_rows(const TreeArgs& a, hipStream_t st) {
   // two tiles a wave: widened records serve both (16 drafts 66 us, 99 with
   // one); row waves that hold the same records as far as 16 drafts (12 in 64
   // paged sequences of 2000 keys 72 us, 80 when they are widened once into
-  // LDS), widened once past them (32 drafts 93 us, 122 by 4 row waves each for
+  // LDS), widened once past them (32 drafts 93 us then, 122 by 4 row waves each for
   // itself; 64 drafts 154 us, 219 by 8)
   else if (tiles <= 2) hipLaunchKernelGGL((k_tree<F, 2, 1, 8, PAGED>), grid, dim3(512), 0, st, a);
   else if (tiles <= 4) hipLaunchKernelGGL((k_tree<F, 2, 2, 4, PAGED>), grid, dim3(512), 0, st, a);
