@@ -35,9 +35,9 @@ def spoil(cache, b, g, slot, dim):
         row[256 + dim // 32] = 255
 
 
-# blocks of a sequence: 3 (31 x 3 x 4 = 372 are cut, 32 x 3 x 4 = 384 are not), 4, 2, 1 with many sequences
-@pytest.mark.parametrize("batch,n", [(31, 130), (32, 140), (33, 200), (49, 65)])
-@pytest.mark.parametrize("window,sink,cap", [(None, 0, 0.0), (70, 6, 0.0), (33, 40, 9.0)])
+# blocks of a sequence: 3 (31 x 3 x 4 = 372 are cut, 32 x 3 x 4 = 384 are not) and 2
+@pytest.mark.parametrize("batch,n", [(31, 130), (32, 140), (49, 65)])
+@pytest.mark.parametrize("window,sink,cap", [(None, 0, 9.0), (70, 6, 0.0)])
 @pytest.mark.parametrize("page_tokens", [0, 16])
 @pytest.mark.parametrize("bits", [8, 4])
 def test_batches_of_prompts(bits, page_tokens, window, sink, cap, batch, n):

@@ -38,13 +38,11 @@ def test_holes_and_nan(bits, window, sink, n):
     verify(cache, queries(5, n), None, counts, 6.0, window, sink)
 
 
-@pytest.mark.parametrize("n", [20, 40])
-@pytest.mark.parametrize("window,sink", [(None, 0), (8000, 70)])
-@pytest.mark.parametrize("page_tokens", [0, 64])
-@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("n,window,sink", [(20, None, 0), (40, None, 0), (40, 8000, 70)])
+@pytest.mark.parametrize("bits,page_tokens", [(8, 0), (8, 64), (4, 64)])
 def test_long_shares(bits, page_tokens, window, sink, n):
-    cache = make([9000, 30, 0], 9000 + n, page_tokens, seed=3, bits=bits)
-    verify(cache, queries(3, n), random_tree(3, n), cap=20.0 if n == 20 else 0.0, window=window, sink=sink)
+    cache = make([9000], 9000 + n, page_tokens, seed=3, bits=bits)
+    verify(cache, queries(1, n), random_tree(1, n), cap=20.0 if n == 20 else 0.0, window=window, sink=sink)
 
 
 @pytest.mark.parametrize("bits,page_tokens", [(8, 0), (8, 16), (4, 16)])
